@@ -16,6 +16,9 @@ using ma_host::fail;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// A launch holds fewer than 2^32 threads; workgroups have at most 512.
+constexpr int64_t kMaxGrid = INT32_MAX / 512;
+
 // What every call needs of a descriptor.
 int check(const ma_paged_desc* d, const char* who) {
   if (!d) return fail("%s: null descriptor", who);
@@ -141,7 +144,7 @@ int ma_paged_append(const ma_paged_desc* d, const void* key, const void* value, 
   a.inter = d->interleaved != 0;
   // positions start anywhere in a page, so one more than the rows alone fill
   const int64_t wgs = key_sums ? (d->num_tokens - 1 + a.step - 1) / a.step + 1 : (d->num_tokens + 63) / 64;
-  if (wgs * d->batch > INT32_MAX) return fail("%s: batch * num_tokens too large", who);
+  if (wgs * d->batch > kMaxGrid) return fail("%s: batch * num_tokens too large", who);
   a.wgs = (int32_t)wgs;
   Events ev(d);
   (void)hipGetLastError();
@@ -207,7 +210,7 @@ int ma_paged_decode(const ma_paged_desc* d, const void* query, const void* cache
   a.nglobal = d->num_global;
   const float scale = d->scale > 0.0f ? d->scale : 1.0f / std::sqrt((float)a.D);
   a.scale_log2 = scale * 1.4426950408889634f;
-  if (d->batch * a.Hkv * a.gt * ns > INT32_MAX || d->batch * a.H > INT32_MAX)
+  if (d->batch * a.Hkv * a.gt * ns > kMaxGrid || d->batch * a.H > kMaxGrid)
     return fail("%s: batch * heads too large", who);
   if (need) {
     a.part_o = static_cast<float*>(workspace);
@@ -252,7 +255,7 @@ int ma_paged_select(const ma_paged_desc* d, const void* query, const float* key_
   a.S = (int32_t)d->num_selected;
   a.first = (int32_t)d->first_pages;
   a.local = (int32_t)d->local_pages;
-  if (d->batch * a.Hkv > INT32_MAX) return fail("%s: batch * heads too large", who);
+  if (d->batch * a.Hkv > kMaxGrid) return fail("%s: batch * heads too large", who);
   Events ev(d);
   (void)hipGetLastError();
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -24,10 +24,13 @@ reached through the converters, as the reference's bridge reaches it.
 
 New, keyword-only constructor arguments select the benchmark patterns and
 default to the reference behaviour: ``pattern`` ("sliding", "dense",
-"block_sparse", "longformer", "index_set"), ``causal``, ``window_left``,
-``window_right``, ``dilation``, ``block_size``, ``block_table``,
-``num_global_tokens``, ``index_set`` (an explicit key set per query row: a
-``sparse_attention_cuda.IndexSet`` or an (offsets, keys) CSR pair).
+"block_sparse", "longformer", "index_set", "block_select"), ``causal``,
+``window_left``, ``window_right``, ``dilation``, ``block_size``,
+``block_table``, ``num_global_tokens``, ``index_set`` (an explicit key set per
+query row: a ``sparse_attention_cuda.IndexSet`` or an (offsets, keys) CSR
+pair), ``num_selected``, ``first_blocks`` and ``local_blocks`` ("block_select":
+each query attends the blocks that ``sparse_attention_cuda.select_blocks`` lists
+for it).
 """
 from __future__ import annotations
 
@@ -68,7 +71,7 @@ except ImportError:  # pragma: no cover - without libma_attn.so
 class PatternSpec:
     """A resolved index-set choice (see include/ma_attn.h for the sets)."""
 
-    pattern: str = "sliding"       # sliding | dense | block_sparse | longformer | index_set
+    pattern: str = "sliding"       # sliding | dense | block_sparse | longformer | index_set | block_select
     left: int = 64
     right: int = 64
     dilation: int = 1
@@ -77,6 +80,9 @@ class PatternSpec:
     block_table: Optional[torch.Tensor] = None
     num_global: int = 0
     index_set: Optional[object] = None  # IndexSet or (offsets, keys)
+    num_selected: int = 0
+    first_blocks: int = 0
+    local_blocks: int = 1
     # device-side forms built on first use and kept: (device, seq_len) ->
     # BlockTable (block_sparse) or IndexSet (index_set given as a CSR pair)
     device_forms: dict = field(default_factory=dict, compare=False, hash=False, repr=False)
@@ -214,14 +220,46 @@ def _native_forward(q, k, v, sparse, window_size, use_causal_mask, spec: Optiona
         return ext.longformer_forward(cq, ck, cv, spec.left, spec.right, spec.num_global)
     if spec.pattern == "index_set":
         return ext.index_set_forward(cq, ck, cv, spec.native_index_set(cq.shape[1], cq.device))
+    if spec.pattern == "block_select":
+        return ext.selected_forward(cq, ck, cv, _native_blocks(cq, ck, spec), spec.block_size, spec.causal)
     raise ValueError(f"unknown pattern {spec.pattern}")
+
+
+def _native_blocks(q, k, spec: PatternSpec) -> torch.Tensor:
+    return sparse_attention_cuda.select_blocks(q, k, spec.num_selected, spec.block_size, spec.causal,
+                                               spec.first_blocks, spec.local_blocks)
+
+
+def _block_select_mask(query, key, spec: PatternSpec) -> torch.Tensor:
+    """[B, H, N, N] keys that select_blocks lists (as it does, in float64)."""
+    B, N, H, D = query.shape
+    bs = spec.block_size
+    nb = (N + bs - 1) // bs
+    with torch.no_grad():
+        blk = torch.arange(N, device=query.device) // bs
+        sums = torch.zeros(B, nb, H, D, dtype=torch.float64, device=query.device).index_add_(1, blk, key.double())
+        mean = sums / torch.bincount(blk, minlength=nb)[None, :, None, None]
+        s = torch.matmul(query.double().transpose(1, 2), mean.permute(0, 2, 3, 1).contiguous())  # [B, H, N, nb]
+        s = torch.where(torch.isnan(s), torch.full_like(s, float("-inf")), s)
+        j, own = torch.arange(nb, device=query.device)[None], blk[:, None]
+        allowed = (j <= own) if spec.causal else (j >= 0).expand(N, nb)
+        forced = allowed & ((j < spec.first_blocks) | ((j <= own) & (j > own - spec.local_blocks)))
+        # best first, ties to the lower block; then the forced ones ahead, the forbidden ones behind
+        order = torch.sort(s, dim=-1, descending=True, stable=True).indices
+        cls = torch.where(forced, 0, torch.where(allowed, 1, 2)).expand(B, H, N, nb)
+        order = order.gather(-1, torch.sort(cls.gather(-1, order), dim=-1, stable=True).indices)
+        hit = torch.zeros_like(s, dtype=torch.bool).scatter_(-1, order[..., :spec.num_selected], True) & allowed
+        mask = hit[..., blk]
+        if spec.causal:
+            mask = mask & torch.ones(N, N, dtype=torch.bool, device=query.device).tril()
+    return mask
 
 
 def pytorch_pattern_attention(query, key, value, spec: PatternSpec) -> torch.Tensor:
     """Differentiable masked attention for any PatternSpec (float32 math)."""
     B, S, H, D = query.shape
     scale = 1.0 / (D ** 0.5)
-    mask = spec.mask(S, query.device)
+    mask = _block_select_mask(query, key, spec) if spec.pattern == "block_select" else spec.mask(S, query.device)
     qh, kh, vh = (t.transpose(1, 2).float() for t in (query, key, value))
     s = torch.matmul(qh * scale, kh.transpose(-2, -1))
     s = s.masked_fill(~mask, float("-inf"))
@@ -235,7 +273,8 @@ class MACoreAttentionFunction(torch.autograd.Function):
     index sets, block-sparse and Longformer on the tiled index-set kernels
     (the latter two as their explicit key sets).  When those sets' tiles
     average more than two entries, the forward also keeps each row's softmax
-    statistic and the backward starts from it and the saved output; the
+    statistic and the backward starts from it and the saved output, as
+    block_select's always does (from the list of its forward too); the
     16-bit Longformer with a causal window of at most 128 keys and 1 to 16
     global tokens then runs the one-pass kernel (longformer_backward).
 
@@ -260,6 +299,14 @@ class MACoreAttentionFunction(torch.autograd.Function):
             if not _HAS_SPARSE_CUDA:
                 raise RuntimeError("device tensors given but the native sparse-attention "
                                    "library (libma_attn.so) is not loaded")
+            if spec is not None and spec.pattern == "block_select" and any(ctx.needs_input_grad[:3]):
+                cq, ck, cv = query.contiguous(), key.contiguous(), value.contiguous()
+                blocks = _native_blocks(cq, ck, spec)
+                out, lse = sparse_attention_cuda.selected_forward(cq, ck, cv, blocks, spec.block_size, spec.causal,
+                                                                  return_lse=True)
+                ctx.saved_plan = ("selected", None)
+                ctx.save_for_backward(query, key, value, out, lse, blocks)
+                return out
             plan = _saved_statistics_plan(spec, sparse, query) if any(ctx.needs_input_grad[:3]) else None
             if plan is not None:
                 try:
@@ -284,15 +331,18 @@ class MACoreAttentionFunction(torch.autograd.Function):
     def backward(ctx, grad_output: torch.Tensor) -> Tuple[Optional[torch.Tensor], ...]:
         query, key, value = ctx.saved_tensors[:3]
         spec = ctx.spec
-        native = spec is None or spec.pattern in ("sliding", "dense", "index_set", "block_sparse", "longformer")
+        native = spec is None or spec.pattern in _PATTERNS
         if _HAS_SPARSE_CUDA and query.is_cuda and native:
             ext = sparse_attention_cuda
             cq, ck, cv, cgo = (t.contiguous() for t in (query, key, value, grad_output))
             cgo = cgo.to(cq.dtype)
             if ctx.saved_plan is not None:  # from the forward's output and statistics
-                out, lse = ctx.saved_tensors[3:]
+                out, lse = ctx.saved_tensors[3:5]
                 kind, iset = ctx.saved_plan
-                if kind == "longformer":
+                if kind == "selected":
+                    dQ, dK, dV = ext.selected_backward(cq, ck, cv, cgo, ctx.saved_tensors[5], spec.block_size,
+                                                       spec.causal, out=out, lse=lse)
+                elif kind == "longformer":
                     dQ, dK, dV = ext.longformer_backward(cq, ck, cv, cgo, spec.left, spec.right, spec.num_global,
                                                          out=out, lse=lse)
                 elif kind == "set":
@@ -398,7 +448,7 @@ def pytorch_sparse_attention(query: torch.Tensor, key: torch.Tensor, value: torc
     return torch.cat(out, dim=1).contiguous()
 
 
-_PATTERNS = ("sliding", "dense", "block_sparse", "longformer", "index_set")
+_PATTERNS = ("sliding", "dense", "block_sparse", "longformer", "index_set", "block_select")
 
 
 class MACoreAttention(nn.Module):
@@ -415,7 +465,8 @@ class MACoreAttention(nn.Module):
                  window_left: Optional[int] = None, window_right: Optional[int] = None,
                  dilation: int = 1, block_size: int = 64,
                  block_table: Optional[torch.Tensor] = None, num_global_tokens: int = 0,
-                 index_set: Optional[object] = None):
+                 index_set: Optional[object] = None, num_selected: int = 0, first_blocks: int = 0,
+                 local_blocks: int = 1):
         super().__init__()
         self.sparse = sparse
         if self.sparse:
@@ -427,9 +478,11 @@ class MACoreAttention(nn.Module):
         self.use_causal_mask = use_causal_mask
         self.fallback_training = fallback_training
         self.spec = self._resolve(pattern, causal, window_left, window_right, dilation,
-                                  block_size, block_table, num_global_tokens, index_set)
+                                  block_size, block_table, num_global_tokens, index_set,
+                                  num_selected, first_blocks, local_blocks)
 
-    def _resolve(self, pattern, causal, left, right, dilation, block_size, table, num_global, index_set):
+    def _resolve(self, pattern, causal, left, right, dilation, block_size, table, num_global, index_set,
+                 num_selected=0, first_blocks=0, local_blocks=1):
         if pattern is None and not causal and left is None and right is None and dilation == 1:
             return None  # reference behaviour
         pattern = pattern or ("sliding" if self.sparse else "dense")
@@ -451,12 +504,20 @@ class MACoreAttention(nn.Module):
             table = torch.as_tensor(table, dtype=torch.int32).cpu()
         if pattern == "index_set" and index_set is None:
             raise ValueError("index_set pattern needs index_set")
-        if pattern == "dense":
+        if pattern == "block_select":
+            if block_size not in (16, 32, 64):
+                raise ValueError("block_select block_size must be 16, 32 or 64")
+            if not 1 <= int(num_selected) <= 64:
+                raise ValueError("block_select needs num_selected in [1, 64]")
+            if first_blocks < 0 or local_blocks < 1 or first_blocks + local_blocks > num_selected:
+                raise ValueError("first_blocks >= 0 and local_blocks >= 1 must fit in num_selected")
+        if pattern in ("dense", "block_select"):
             causal = causal or self.use_causal_mask
         return PatternSpec(pattern=pattern, left=int(left or 0), right=int(right or 0),
                            dilation=int(dilation), causal=bool(causal),
                            block_size=int(block_size), block_table=table,
-                           num_global=int(num_global), index_set=index_set)
+                           num_global=int(num_global), index_set=index_set, num_selected=int(num_selected),
+                           first_blocks=int(first_blocks), local_blocks=int(local_blocks))
 
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> torch.Tensor:
         if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:

@@ -24,6 +24,11 @@ New pattern entry points (not in the reference; the benchmark patterns):
     make_block_table(seed, num_blocks, random_per_row=2)
     index_set_forward(q, k, v, index_set)              (explicit key set per query row)
     IndexSet(offsets, keys, seq_len), IndexSet.from_coo(rows, cols, seq_len)
+    select_blocks(q, k, num_selected, block_size=64)   (the blocks a cheap score selects, per query)
+    selected_forward(q, k, v, blocks), selected_backward(q, k, v, grad_out, blocks, out=, lse=)
+
+The selected ones take keys and values with fewer heads than the queries; their
+single-token forms, over a paged cache, are in ``paged_attention``.
 
 Forward and backward are hand-written HIP kernels (libma_attn.so).  The
 backward recomputes the softmax from q, k, v as the reference's does, for the
@@ -45,7 +50,7 @@ import ma_attn as _ma
 __all__ = ["forward", "dense_forward", "backward", "dense_backward", "sliding_forward",
            "sliding_backward", "block_sparse_forward", "longformer_forward", "longformer_backward",
            "make_block_table", "BlockTable", "IndexSet", "index_set_forward", "index_set_backward",
-           "pattern_index_set"]
+           "pattern_index_set", "select_blocks", "selected_forward", "selected_backward"]
 
 
 def _check(*ts: torch.Tensor) -> None:
@@ -581,3 +586,143 @@ def sliding_backward(query, key, value, grad_out, left: int, right: int,
     """dQ, dK, dV of sliding_forward() (keys {i + dilation*t : -left <= t <= right})."""
     return _backward(query, key, value, grad_out, _ma.SLIDING, left=int(left), right=int(right),
                      dilation=int(dilation))
+
+
+# ---------------------------------------------------------------- selected blocks
+
+class _SelectDesc(ctypes.Structure):
+    """Mirror of ``ma_select_desc`` (include/ma_select.h)."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in (
+        "batch", "seq_len", "num_heads", "num_kv_heads", "head_dim", "block_size", "num_selected")]
+    _fields_ += [("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("first_blocks", ctypes.c_int64),
+                 ("local_blocks", ctypes.c_int64), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+                 ("start_event", ctypes.c_void_p), ("stop_event", ctypes.c_void_p)]
+
+
+for _name, _nptr in (("select_blocks", 3), ("selected_forward", 6), ("selected_backward", 10)):
+    _f = getattr(_ma.LIB, "ma_" + _name)
+    _f.restype = ctypes.c_int
+    _f.argtypes = [ctypes.POINTER(_SelectDesc)] + [ctypes.c_void_p] * (_nptr + 1) + [ctypes.c_size_t, ctypes.c_void_p]
+    _f = getattr(_ma.LIB, f"ma_{_name}_workspace_size")
+    _f.restype = ctypes.c_size_t
+    _f.argtypes = [ctypes.POINTER(_SelectDesc)]
+
+
+def _check_selected(q: torch.Tensor, *kv: torch.Tensor) -> None:
+    """q [B, S, H, D], the others [B, S, Hkv, D] with H a multiple of Hkv."""
+    for t in (q, *kv):
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError("Inputs must be tensors")
+        if not t.is_cuda:
+            raise RuntimeError("Inputs must be CUDA (HIP) device tensors")
+        if t.dtype != q.dtype or t.dtype not in _ma.DTYPES:
+            raise RuntimeError("Inputs must share one dtype among float32, bfloat16, float16")
+        if not t.is_contiguous():
+            raise RuntimeError("Inputs must be contiguous")
+        if t.dim() != 4:
+            raise RuntimeError("Expected shape [B, S, H, D]")
+        if t.device != q.device:
+            raise RuntimeError("Inputs must be on one device")
+        if t.shape != kv[0].shape:
+            if t is not q:
+                raise RuntimeError("K,V must have same shape")
+    B, N, H, D = q.shape
+    Bk, Nk, Hkv, Dk = kv[0].shape
+    if (B, N, D) != (Bk, Nk, Dk):
+        raise RuntimeError("Q,K,V must have the same batch, sequence length and head_dim")
+    if Hkv < 1 or H < 1 or H % Hkv:
+        raise RuntimeError(f"query heads ({H}) must be a multiple of key/value heads ({Hkv})")
+
+
+def _select_desc(q, k, block_size, num_selected, causal, **kw):
+    B, N, H, D = q.shape
+    d = _SelectDesc(batch=B, seq_len=N, num_heads=H, num_kv_heads=k.shape[2], head_dim=D, block_size=int(block_size),
+                    num_selected=int(num_selected), dtype=_ma.DTYPES[q.dtype], causal=int(bool(causal)), **kw)
+    if _events is not None:
+        d.start_event, d.stop_event = (e or None for e in _events)
+    return d
+
+
+def _call_selected(name: str, d: _SelectDesc, dev: int, device, *ptrs) -> None:
+    nbytes = int(getattr(_ma.LIB, f"ma_{name}_workspace_size")(ctypes.byref(d)))
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    args = [p.data_ptr() or None if isinstance(p, torch.Tensor) else p for p in ptrs]
+    fn = getattr(_ma.LIB, "ma_" + name)
+    if _on_device(dev, lambda stream: fn(ctypes.byref(d), *args, ws.data_ptr(), nbytes, stream or None)) != 0:
+        raise RuntimeError(_ma.last_error())
+
+
+def select_blocks(query: torch.Tensor, key: torch.Tensor, num_selected: int, block_size: int = 64,
+                  causal: bool = True, first_blocks: int = 0, local_blocks: int = 1) -> torch.Tensor:
+    """The key blocks each query attends: for query [B, S, H, D] and key
+    [B, S, Hkv, D] the num_selected (at most 64) blocks of block_size (16, 32 or
+    64) keys whose mean has the largest dot product with the sum of a key/value
+    head's queries -> int32 [B, S, Hkv, num_selected], ascending, -1 behind them.
+
+    causal: blocks up to the query's own.  The first ``first_blocks`` blocks, the
+    query's own and the ``local_blocks`` - 1 before it are always listed.  Scores
+    are float64; ties go to the lower block and NaN scores rank last.  The list is
+    no function of the inputs to differentiate: gradients flow through
+    selected_forward's keys and queries only.  At most 16384 blocks.
+    """
+    _check_selected(query, key)
+    S, first, local = int(num_selected), int(first_blocks), int(local_blocks)
+    if not 1 <= S <= 64:
+        raise RuntimeError("num_selected must be in [1, 64]")
+    if first < 0 or local < 1 or first + local > S:
+        raise RuntimeError("first_blocks >= 0 and local_blocks >= 1 must fit in num_selected")
+    d = _select_desc(query, key, block_size, S, causal, first_blocks=first, local_blocks=local)
+    B, N, Hkv, _ = key.shape
+    out = torch.empty((B, N, Hkv, S), dtype=torch.int32, device=query.device)
+    _call_selected("select_blocks", d, query.get_device(), query.device, query, key, out)
+    return out
+
+
+def _check_blocks(blocks, key) -> None:
+    B, N, Hkv, _ = key.shape
+    if not (isinstance(blocks, torch.Tensor) and blocks.dtype == torch.int32 and blocks.is_contiguous()
+            and blocks.device == key.device and blocks.dim() == 4 and tuple(blocks.shape[:3]) == (B, N, Hkv)
+            and 1 <= blocks.shape[3] <= 64):
+        raise RuntimeError(f"blocks must be a contiguous int32 [{B}, {N}, {Hkv}, n] tensor with 1 <= n <= 64 "
+                           "on the inputs' device")
+
+
+def selected_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, blocks: torch.Tensor,
+                     block_size: int = 64, causal: bool = True, return_lse: bool = False, scale=None):
+    """Each query attends the keys of its own listed blocks (select_blocks'
+    layout), up to itself when causal.  Entries outside the sequence, blocks
+    behind the query (causal) and repeats are skipped; a query without keys gives
+    zeros.  Key/value heads may be fewer than query heads.  return_lse: also
+    float32 [B, S, H], log2 of the sum of exp(scaled scores) (-inf without keys),
+    for selected_backward(..., out=, lse=).  scale: softmax scale (None:
+    1/sqrt(head_dim)).  The workspace holds a float32 row of head_dim per query
+    head and listed block, for as many key/value heads as fit in 1 GiB (at least
+    one)."""
+    _check_selected(query, key, value)
+    _check_blocks(blocks, key)
+    d = _select_desc(query, key, block_size, blocks.shape[3], causal, **_scale_kw(scale))
+    out = torch.empty_like(query)
+    lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device) if return_lse else None
+    _call_selected("selected_forward", d, query.get_device(), query.device, query, key, value, blocks, out, lse)
+    return (out, lse) if return_lse else out
+
+
+def selected_backward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, grad_out: torch.Tensor,
+                      blocks: torch.Tensor, block_size: int = 64, causal: bool = True, out=None, lse=None,
+                      scale=None) -> List[torch.Tensor]:
+    """dQ, dK, dV of selected_forward for a given list.  out, lse: the forward's
+    output and statistics (return_lse=True); without both the forward runs again
+    here."""
+    _check_selected(query, key, value)
+    _check_blocks(blocks, key)
+    _check(query, grad_out)
+    if out is None or lse is None:
+        out, lse = selected_forward(query, key, value, blocks, block_size, causal, True, scale)
+    _check(query, out)
+    _check_lse(lse, query)
+    d = _select_desc(query, key, block_size, blocks.shape[3], causal, **_scale_kw(scale))
+    dq, dk, dv = (torch.empty_like(t) for t in (query, key, value))
+    _call_selected("selected_backward", d, query.get_device(), query.device, query, key, value, blocks, out, lse,
+                   grad_out, dq, dk, dv)
+    return [dq, dk, dv]
