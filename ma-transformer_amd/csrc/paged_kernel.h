@@ -71,9 +71,13 @@ struct Vec8 {
   }
 };
 
+// Through float32, as torch converts float64 (the compiler would fold the two
+// conversions to f16 into one).
 template <typename T>
 __device__ __forceinline__ T round_to(double y) {
-  return static_cast<T>(static_cast<float>(y));
+  float f = static_cast<float>(y);
+  asm volatile("" : "+v"(f));
+  return static_cast<T>(f);
 }
 
 // Rotates the row at src (head_dim D, R of it rotated) into dst, one unit of

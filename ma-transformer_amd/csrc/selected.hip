@@ -101,7 +101,7 @@ int place(Layout& l, const ma_select_desc* d, void* ws, size_t bytes, const char
 int check_grids(const Layout& l, const char* who) {
   const Args& a = l.a;
   const int64_t lim = INT32_MAX / 1024;
-  if (l.units * a.chunks > lim || l.group * (int64_t)a.max_items > lim || l.group * (int64_t)a.nb > lim ||
+  if (l.units * a.chunks > lim || l.group * (int64_t)a.max_items > lim || l.group * (int64_t)a.nb * kKvParts > lim ||
       l.group * a.N * a.G / kJoinWaves > lim || (int64_t)a.N * a.S > INT32_MAX ||
       l.units / a.Hkv * a.N * a.H / 32 > lim)
     return fail("%s: batch * seq_len * heads too large", who);
@@ -110,16 +110,20 @@ int check_grids(const Layout& l, const char* who) {
 
 int build_lists(const Layout& l, hipStream_t st) {
   const Args& a = l.a;
-  const size_t bm = (size_t)a.nb * a.words * 8, tot = (size_t)a.nb * 4;
-  if (bm > 48 * 1024 && (ma_host::reserve_lds(reinterpret_cast<const void*>(&count_kernel), kMaxBlocks * 8, st) ||
-                         ma_host::reserve_lds(reinterpret_cast<const void*>(&fill_kernel), kMaxBlocks * 8, st)))
+  const size_t bm = (size_t)a.nb * a.words * 8, tot = (size_t)a.nb * 4, fill = fill_lds_bytes(a.nb, a.words, a.S);
+  static_assert(kMaxBlocks * 8 + 64 * 64 * 4 <= 160 * 1024 && 2048 * (4 * 8 + 4) + 256 * 64 * 4 <= 160 * 1024,
+                "fill_kernel's LDS");
+  if (bm > 48 * 1024 && ma_host::reserve_lds(reinterpret_cast<const void*>(&count_kernel), kMaxBlocks * 8, st))
+    return 1;
+  if (fill > 48 * 1024 &&
+      ma_host::reserve_lds(reinterpret_cast<const void*>(&fill_kernel), kMaxBlocks * 8 + 64 * 64 * 4, st))
     return 1;
   if (tot > 48 * 1024 && ma_host::reserve_lds(reinterpret_cast<const void*>(&scan_kernel), kMaxBlocks * 4, st))
     return 1;
   const dim3 grid((unsigned)(l.units * a.chunks));
   ma_host::launch(false, count_kernel, grid, dim3(kListThreads), (uint32_t)bm, st, a);
   ma_host::launch(false, scan_kernel, dim3((unsigned)l.units), dim3(kScanThreads), (uint32_t)tot, st, a);
-  ma_host::launch(false, fill_kernel, grid, dim3(kListThreads), (uint32_t)bm, st, a);
+  ma_host::launch(false, fill_kernel, grid, dim3(kListThreads), (uint32_t)fill, st, a);
   return 0;
 }
 
@@ -162,7 +166,7 @@ int backward_dn(Layout l, hipStream_t st) {
     a.units = (int32_t)std::min(l.group, l.units - u);
     ma_host::launch(false, backward_kernel<T, DP, NT>, dim3((unsigned)(a.units * a.max_items)), dim3(64 * NT),
                     (uint32_t)shm, st, a);
-    ma_host::launch(false, join_kv_kernel<T>, dim3((unsigned)(a.units * a.nb)), dim3(256), 0, st, a);
+    ma_host::launch(false, join_kv_kernel<T>, dim3((unsigned)(a.units * a.nb * kKvParts)), dim3(256), 0, st, a);
     join<T, false>(a, u + l.group >= l.units, st);
   }
   return launched("ma_selected_backward");

@@ -72,24 +72,21 @@ __device__ __forceinline__ const int32_t* row_of(const Args& a, int unit, int64_
   return a.blocks + (((int64_t)(unit / a.Hkv) * a.N + i) * a.Hkv + unit % a.Hkv) * a.S;
 }
 
-__device__ __forceinline__ void mark_chunk(const Args& a, int unit, int64_t q0, unsigned long long* bm) {
+__global__ __launch_bounds__(kListThreads) void count_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  unsigned long long* bm = reinterpret_cast<unsigned long long*>(lds);
+  const uint32_t x = (uint32_t)xcd_row_order((int)blockIdx.x, (int)gridDim.x);
+  const int unit = x / (uint32_t)a.chunks, ch = x % (uint32_t)a.chunks;
+  const int64_t q0 = (int64_t)ch * 64 * a.words;
+  const int nq = (int)(a.N - q0 < 64 * a.words ? a.N - q0 : 64 * a.words);
   for (int i = threadIdx.x; i < a.nb * a.words; i += kListThreads) bm[i] = 0;
   __syncthreads();
-  const int nq = 64 * a.words;
   for (int e = threadIdx.x; e < nq * a.S; e += kListThreads) {
     const int qi = e / a.S, j = e - qi * a.S;
-    if (q0 + qi >= a.N) break;
     const int b = listed(a, row_of(a, unit, q0 + qi), q0 + qi, j);
     if (b >= 0) atomicOr(&bm[b * a.words + (qi >> 6)], 1ull << (qi & 63));
   }
   __syncthreads();
-}
-
-__global__ __launch_bounds__(kListThreads) void count_kernel(Args a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  unsigned long long* bm = reinterpret_cast<unsigned long long*>(lds);
-  const int unit = blockIdx.x / (uint32_t)a.chunks, ch = blockIdx.x % (uint32_t)a.chunks;
-  mark_chunk(a, unit, (int64_t)ch * 64 * a.words, bm);
   uint32_t* out = a.counts + ((int64_t)unit * a.chunks + ch) * a.nb;
   for (int b = threadIdx.x; b < a.nb; b += kListThreads) {
     uint32_t n = 0;
@@ -161,24 +158,44 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(Args a) {
   for (int i = (int)total + tid; i < a.max_items; i += kScanThreads) it[i] = make_int4(0, 0, -1, 0);
 }
 
+// dynamic LDS of fill_kernel: the bitmap, the chunk's rows, and (small tables)
+// where each block's pairs of this chunk begin
+inline size_t fill_lds_bytes(int nb, int words, int S) {
+  return (size_t)nb * words * 8 + (size_t)64 * words * S * 4 + (words > 1 ? (size_t)nb * 4 : 0);
+}
+
 __global__ __launch_bounds__(kListThreads) void fill_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   unsigned long long* bm = reinterpret_cast<unsigned long long*>(lds);
-  const int unit = blockIdx.x / (uint32_t)a.chunks, ch = blockIdx.x % (uint32_t)a.chunks;
+  int32_t* rows = reinterpret_cast<int32_t*>(bm + a.nb * a.words);
+  uint32_t* begin = reinterpret_cast<uint32_t*>(rows + 64 * a.words * a.S);
+  const uint32_t x = (uint32_t)xcd_row_order((int)blockIdx.x, (int)gridDim.x);
+  const int unit = x / (uint32_t)a.chunks, ch = x % (uint32_t)a.chunks;
   const int64_t q0 = (int64_t)ch * 64 * a.words;
-  mark_chunk(a, unit, q0, bm);
+  const int nq = (int)(a.N - q0 < 64 * a.words ? a.N - q0 : 64 * a.words);
   const uint32_t* base = a.counts + ((int64_t)unit * a.chunks + ch) * a.nb;
-  int32_t* list = a.list + (int64_t)unit * a.N * a.S;
-  for (int e = threadIdx.x; e < 64 * a.words * a.S; e += kListThreads) {
+  const int32_t* offs = a.offs + (int64_t)unit * a.nb;
+  const bool staged = a.words > 1;
+  if (staged)
+    for (int i = threadIdx.x; i < a.nb; i += kListThreads) begin[i] = base[i] + (uint32_t)offs[i];
+  for (int i = threadIdx.x; i < a.nb * a.words; i += kListThreads) bm[i] = 0;
+  __syncthreads();
+  for (int e = threadIdx.x; e < nq * a.S; e += kListThreads) {
     const int qi = e / a.S, j = e - qi * a.S;
-    if (q0 + qi >= a.N) break;
-    const int32_t* row = row_of(a, unit, q0 + qi);
-    const int b = listed(a, row, q0 + qi, j);
+    const int b = listed(a, row_of(a, unit, q0 + qi), q0 + qi, j);
+    rows[e] = b;
+    if (b >= 0) atomicOr(&bm[b * a.words + (qi >> 6)], 1ull << (qi & 63));
+  }
+  __syncthreads();
+  int32_t* list = a.list + (int64_t)unit * a.N * a.S;
+  for (int e = threadIdx.x; e < nq * a.S; e += kListThreads) {
+    const int b = rows[e];
     if (b < 0) continue;
+    const int qi = e / a.S, j = e - qi * a.S;
     bool again = false;  // an earlier entry of the row is this block
-    for (int i = 0; i < j; ++i) again = again || row[i] == b;
+    for (int i = 0; i < j; ++i) again = again || rows[e - j + i] == b;
     if (again) continue;
-    uint32_t rank = base[b] + (uint32_t)a.offs[(int64_t)unit * a.nb + b];
+    uint32_t rank = staged ? begin[b] : base[b] + (uint32_t)offs[b];
     for (int w = 0; w < (qi >> 6); ++w) rank += (uint32_t)__popcll(bm[b * a.words + w]);
     rank += (uint32_t)__popcll(bm[b * a.words + (qi >> 6)] & ((1ull << (qi & 63)) - 1));
     list[rank] = (int32_t)((q0 + qi) * 64 + j);
@@ -198,30 +215,40 @@ __global__ __launch_bounds__(kListThreads) void fill_kernel(Args a) {
 
 constexpr int kFwdWaves = 4;
 
-// Value rows 4 g + i of a 16-key tile, elements VPL c .. of each, as the words
-// the lane loads, and the V^T operands built from two such tiles.
+// Value rows 4 g + i of a 16-key tile as the words the lane loads, and the V^T
+// operands built from two such tiles.  Lane column c takes the 4 (VPL = 2: 2)
+// elements at 4 p(c), p(c) = 4 (c % 4) + c / 4, of each 64 (32): a result's rows
+// 4 g + y are then elements at 4 (4 y + g), and the four lanes that share a row
+// store 64 contiguous bytes at once.
 template <typename T, int DP>
 struct ValueRows {
   static constexpr int VPL = DP / 16;
   static constexpr int VW = VPL * (int)sizeof(T) / 4;
   uint32_t w[4][VW];
+  static constexpr int CH = VPL < 4 ? VPL : 4;        // elements of a chunk
+  static constexpr int CW = CH * (int)sizeof(T) / 4;  // words of it
   __device__ __forceinline__ void load(int i, const T* row, bool ok, int c, int D) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(row + (c * VPL < D ? c * VPL : 0));
-    ok = ok && c * VPL < D;
-    if constexpr (VW == 1) {
-      w[i][0] = p[0];
-    } else if constexpr (VW == 2) {
-      const uint2 x = *reinterpret_cast<const uint2*>(p);
-      w[i][0] = x.x, w[i][1] = x.y;
-    } else {
 #pragma unroll
-      for (int y = 0; y < VW; y += 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(p + y);
-        w[i][y] = x.x, w[i][y + 1] = x.y, w[i][y + 2] = x.z, w[i][y + 3] = x.w;
+    for (int h = 0; h < VPL / CH; ++h) {
+      const int d = 16 * CH * h + CH * (4 * (c & 3) + (c >> 2));
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(row + (d < D ? d : 0));
+      const bool in = ok && d < D;
+      if constexpr (CW == 1) {
+        w[i][h] = p[0];
+      } else if constexpr (CW == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[i][2 * h] = x.x, w[i][2 * h + 1] = x.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[i][4 * h] = x.x, w[i][4 * h + 1] = x.y, w[i][4 * h + 2] = x.z, w[i][4 * h + 3] = x.w;
       }
-    }
 #pragma unroll
-    for (int y = 0; y < VW; ++y) w[i][y] = ok ? w[i][y] : 0u;
+      for (int y = 0; y < CW; ++y) w[i][CW * h + y] = in ? w[i][CW * h + y] : 0u;
+    }
+  }
+  // the head_dim element of result row 4 g + y of operand j
+  static __device__ __forceinline__ int element(int g, int y, int j) {
+    return 16 * CH * (j / CH) + CH * (4 * y + g) + j % CH;
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -231,7 +258,7 @@ struct ValueRows {
   }
 };
 
-// The operand of element j (head_dim VPL c + j) from the tiles u0 and u1.
+// Operand j from the tiles u0 and u1.
 template <typename T, int DP>
 __device__ __forceinline__ typename Op<T>::F value_operand(const ValueRows<T, DP>& u0, const ValueRows<T, DP>& u1, int j) {
   if constexpr (sizeof(T) == 2) {
@@ -250,8 +277,16 @@ __device__ __forceinline__ typename Op<T>::F value_operand(const ValueRows<T, DP
 
 __device__ __forceinline__ int wave_any(bool x) { return __ballot(x) != 0; }
 
+// Waves per SIMD that the registers are budgeted for; two or more keep the
+// products out of the accumulation registers, whose copies cost as much as the
+// products themselves.
 template <typename T, int DP, int NT>
-__global__ __launch_bounds__(64 * kFwdWaves) void forward_kernel(Args a) {
+constexpr int kFwdOcc = DP * NT * (int)sizeof(T) > 512 ? (DP * NT * (int)sizeof(T) > 1024 ? 1 : 2) : 3;
+template <typename T, int DP, int NT>
+constexpr int kBwdOcc = DP > 64 || (sizeof(T) == 4 && DP == 64 && NT == 1) ? 1 : (sizeof(T) == 2 && NT > 1 ? 3 : 2);
+
+template <typename T, int DP, int NT>
+__global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_kernel(Args a) {
   using O = Op<T>;
   using F = typename O::F;
   using W = WeightPlanes<T>;
@@ -308,19 +343,21 @@ __global__ __launch_bounds__(64 * kFwdWaves) void forward_kernel(Args a) {
   // a row past the end repeats the last one and is not stored
   auto entry_of = [&](int r) { return list[(a.G == 1 ? r : r / a.G)]; };
   auto head_of = [&](int r) { return a.G == 1 ? 0 : r % a.G; };
+  auto clamp = [&](int r) { return r < rows ? r : rows - 1; };
+  // a tile's pairs are read two tiles ahead, its queries one
+  constexpr int STEP = 16 * kFwdWaves;
   F qf[NK];
-  int r = 16 * w + c < rows ? 16 * w + c : rows - 1;
-  int ent = entry_of(r), gh = head_of(r);
+  int ent = entry_of(clamp(16 * w + c)), gh = head_of(clamp(16 * w + c));
+  int entn = entry_of(clamp(16 * w + c + STEP));
   auto load_q = [&](F(&f)[NK], int e, int h) {
     const T* p = qp + ((int64_t)(e >> 6) * a.H + h) * D;
 #pragma unroll
     for (int i = 0; i < NK; ++i) f[i] = 32 * i + 8 * g < D ? O::load(p + 32 * i + 8 * g) : O::zero();
   };
   load_q(qf, ent, gh);
-  for (int t0 = 16 * w; t0 < rows; t0 += 16 * kFwdWaves) {
-    const int tn = t0 + 16 * kFwdWaves + c;
-    const int rn = tn < rows ? tn : rows - 1;
-    const int entn = entry_of(rn), ghn = head_of(rn);
+  for (int t0 = 16 * w; t0 < rows; t0 += STEP) {
+    const int ghn = head_of(clamp(t0 + STEP + c));
+    const int ent2 = entry_of(clamp(t0 + 2 * STEP + c));
     f32x4 s[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -391,7 +428,7 @@ __global__ __launch_bounds__(64 * kFwdWaves) void forward_kernel(Args a) {
         for (int y = 0; y < 4; ++y)
 #pragma unroll
           for (int j = 0; j < VPL; ++j) {
-            const int d = (4 * g + y) * VPL + j;
+            const int d = VR::element(g, y, j);
             if (key < lim && d < D) acc[j][y] += pk * (float)row[d];
           }
       }
@@ -400,20 +437,20 @@ __global__ __launch_bounds__(64 * kFwdWaves) void forward_kernel(Args a) {
       const int64_t at = (qi * a.S + (ent & 63)) * a.G + gh;
       float* po = part + at * D;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int d = (4 * g + y) * VPL;
-        if (d >= D) continue;
-        if constexpr (VPL == 2) {
-          *reinterpret_cast<float2*>(po + d) = make_float2(acc[0][y], acc[1][y]);
-        } else {
+      for (int y = 0; y < 4; ++y)
 #pragma unroll
-          for (int j = 0; j < VPL; j += 4)
-            *reinterpret_cast<float4*>(po + d + j) = make_float4(acc[j][y], acc[j + 1][y], acc[j + 2][y], acc[j + 3][y]);
+        for (int j = 0; j < VPL; j += VR::CH) {
+          const int d = VR::element(g, y, j);
+          if (d >= D) continue;
+          if constexpr (VPL == 2)
+            *reinterpret_cast<float2*>(po + d) = make_float2(acc[0][y], acc[1][y]);
+          else
+            *reinterpret_cast<float4*>(po + d) = make_float4(acc[j][y], acc[j + 1][y], acc[j + 2][y], acc[j + 3][y]);
         }
-      }
       if (g == 0) ml[at] = make_float2(m, l);
     }
     ent = entn;
+    entn = ent2;
     gh = ghn;
   }
 }
@@ -553,14 +590,14 @@ struct BwdLds {
   static constexpr int kG = RT * RS;
   static constexpr int kS = 2 * RT * RS;
   static constexpr int kSPlane = 16 * NT * SS;
-  static constexpr int kStat = kS + WeightPlanes<T>::N * kSPlane;  // lse, delta [32], query [32]
+  static constexpr int kStat = kS + WeightPlanes<T>::N * kSPlane;  // lse, delta, pair [32]
   static constexpr int kMax = kStat + 3 * RT * 4;                  // [NT] per-wave maxima
   static constexpr int kFlag = kMax + NT * 4;                      // [2] tile flags, block flag
   static constexpr int kBytes = kFlag + 16;
 };
 
 template <typename T, int DP, int NT>
-__global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
+__global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   using O = Op<T>;
   using F = typename O::F;
@@ -625,11 +662,23 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
   const float* lse = a.lse_in + (int64_t)b * a.N * a.H + (int64_t)hk * a.G;
   const float* dl = a.delta + (int64_t)b * a.N * a.H + (int64_t)hk * a.G;
 
-  // staging: chunk n of a thread is 8 elements of row (tid + n TH) / CPR
+  // staging: chunk n of a thread is 8 elements of row (tid + n TH) / CPR; a
+  // tile's pairs are read two tiles ahead, its rows one
   F sq[NC], sg[NC];
+  int en[NC], est = 0;
   int sflag = 0;
   float s_lse = INFINITY, s_dl = 0.0f;
-  int s_qi = 0;
+  int s_ent = 0;
+  auto pair_of = [&](int rr) { return list[a.G == 1 ? rr : rr / a.G]; };
+  auto head_of = [&](int rr) { return a.G == 1 ? 0 : rr % a.G; };
+  auto pairs = [&](int r0) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int rr = r0 + (tid + n * TH) / CPR;
+      en[n] = pair_of(rr < rows ? rr : rows - 1);
+    }
+    if (tid < RT) est = pair_of(r0 + tid < rows ? r0 + tid : rows - 1);
+  };
   auto fetch = [&](int r0) {
     sflag = 0;
 #pragma unroll
@@ -637,8 +686,7 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
       const int ch = tid + n * TH, rr = r0 + ch / CPR, d = (ch % CPR) * 8;
       sq[n] = sg[n] = O::zero();
       if (ch < RT * CPR && rr < rows && d < D) {
-        const int e = list[a.G == 1 ? rr : rr / a.G];
-        const int64_t at = ((int64_t)(e >> 6) * a.H + (a.G == 1 ? 0 : rr % a.G)) * D + d;
+        const int64_t at = ((int64_t)(en[n] >> 6) * a.H + head_of(rr)) * D + d;
         sq[n] = O::load(qp + at);
         sg[n] = O::load(gp + at);
       }
@@ -646,13 +694,11 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
     if (tid < RT) {
       s_lse = INFINITY;  // a row past the end has no weight
       s_dl = 0.0f;
-      s_qi = 0;
+      s_ent = est;
       if (r0 + tid < rows) {
-        const int rr = r0 + tid, e = list[a.G == 1 ? rr : rr / a.G];
-        const int64_t at = (int64_t)(e >> 6) * a.H + (a.G == 1 ? 0 : rr % a.G);
+        const int64_t at = (int64_t)(est >> 6) * a.H + head_of(r0 + tid);
         s_lse = lse[at];
         s_dl = dl[at];
-        s_qi = e >> 6;
       }
     }
   };
@@ -664,10 +710,14 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
   const float sl2 = a.scale_log2;
   float* st_lse = reinterpret_cast<float*>(lds + L::kStat);
   float* st_dl = st_lse + RT;
-  int* st_qi = reinterpret_cast<int*>(st_dl + RT);
+  int* st_ent = reinterpret_cast<int*>(st_dl + RT);
   float* wmax = reinterpret_cast<float*>(lds + L::kMax);
 
-  if (rows > 0) fetch(0);
+  if (rows > 0) {
+    pairs(0);
+    fetch(0);
+    pairs(RT);
+  }
   int turn = 0;
   for (int r0 = 0; r0 < rows; r0 += RT, turn ^= 1) {
     __syncthreads();  // the last tile has been read
@@ -683,16 +733,19 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
     if (tid < RT) {
       st_lse[tid] = s_lse;
       st_dl[tid] = s_dl;
-      st_qi[tid] = s_qi;
+      st_ent[tid] = s_ent;
       // a row inside the block has keys that it may not see
-      if (a.causal && r0 + tid < rows && s_qi - k0 < nk - 1) sflag |= 1;
+      if (a.causal && r0 + tid < rows && (s_ent >> 6) - k0 < nk - 1) sflag |= 1;
     }
     if (sflag) atomicOr(&flags[turn], sflag);
     if (tid == 0) flags[turn ^ 1] = 0;
     __syncthreads();
     const int fl = flags[turn];
     const bool slow = (fl & 1) && ((fl & 2) || flags[2]);
-    if (r0 + RT < rows) fetch(r0 + RT);
+    if (r0 + RT < rows) {
+      fetch(r0 + RT);
+      pairs(r0 + 2 * RT);
+    }
 
     float p[2][4], ds[2][4];
     bool ok[2][4];
@@ -709,9 +762,9 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
       settle(dp);
       const float4 rl = *reinterpret_cast<const float4*>(st_lse + 16 * u + 4 * g);
       const float4 rd = *reinterpret_cast<const float4*>(st_dl + 16 * u + 4 * g);
-      const int4 rq = *reinterpret_cast<const int4*>(st_qi + 16 * u + 4 * g);
+      const int4 rq = *reinterpret_cast<const int4*>(st_ent + 16 * u + 4 * g);
       const float le[4] = {rl.x, rl.y, rl.z, rl.w}, de[4] = {rd.x, rd.y, rd.z, rd.w};
-      const int qi[4] = {rq.x, rq.y, rq.z, rq.w};
+      const int qi[4] = {rq.x >> 6, rq.y >> 6, rq.z >> 6, rq.w >> 6};
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         ok[u][y] = key < nk && (!a.causal || k0 + key <= qi[y]) && r0 + 16 * u + 4 * g + y < rows;
@@ -855,7 +908,7 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
 #pragma unroll
           for (int pl = W::N - 1; pl >= 0; --pl)
             d1 += (float)*reinterpret_cast<const T*>(lds + L::kS + pl * L::kSPlane + kk * L::SS + (16 * u + c) * (int)sizeof(T));
-          if (k0 + kk > st_qi[16 * u + c]) continue;
+          if (k0 + kk > st_ent[16 * u + c] >> 6) continue;
 #pragma unroll
           for (int i = 0; i < JD; ++i)
 #pragma unroll
@@ -866,7 +919,7 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
         }
       }
       if (rr < rows) {
-        const int e = list[a.G == 1 ? rr : rr / a.G], gh = a.G == 1 ? 0 : rr % a.G;
+        const int e = st_ent[16 * u + c], gh = head_of(rr);
         float* po = part + (((int64_t)(e >> 6) * a.S + (e & 63)) * a.G + gh) * D;
 #pragma unroll
         for (int i = 0; i < JD; ++i) {
@@ -912,17 +965,21 @@ __global__ __launch_bounds__(64 * NT) void backward_kernel(Args a) {
   }
 }
 
-// The parts of a block with more than one item, added in list order.
+// The parts of a block with more than one item, added in list order by
+// kKvParts workgroups.
+constexpr int kKvParts = 8;
+
 template <typename T>
 __global__ __launch_bounds__(256) void join_kv_kernel(Args a) {
-  const int ug = blockIdx.x / (uint32_t)a.nb, blk = blockIdx.x % (uint32_t)a.nb, unit = a.unit0 + ug;
+  const uint32_t x = blockIdx.x / (uint32_t)kKvParts;
+  const int ug = x / (uint32_t)a.nb, blk = x % (uint32_t)a.nb, unit = a.unit0 + ug;
   const int2 bi = a.blk_items[(int64_t)unit * a.nb + blk];
   if (bi.y == 1) return;
   const int b = unit / a.Hkv, hk = unit % a.Hkv, D = a.D, q4 = D >> 2;
   const int64_t k0 = (int64_t)blk * a.BS, rs = (int64_t)a.Hkv * D;
   const int nk = (int)(a.N - k0 < a.BS ? a.N - k0 : a.BS);
   const float* p0 = a.part_kv + ((int64_t)ug * a.max_items + bi.x) * 2 * a.BS * D;
-  for (int e = threadIdx.x; e < 2 * a.BS * q4; e += 256) {
+  for (int e = blockIdx.x % (uint32_t)kKvParts * 256 + threadIdx.x; e < 2 * a.BS * q4; e += 256 * kKvParts) {
     const int m = e / (a.BS * q4), r = e - m * a.BS * q4, key = r / q4, d = 4 * (r - key * q4);
     if (key >= nk) continue;
     float4 s = make_float4(0, 0, 0, 0);
