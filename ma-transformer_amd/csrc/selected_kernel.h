@@ -283,6 +283,8 @@ __device__ __forceinline__ int wave_any(bool x) { return __ballot(x) != 0; }
 template <typename T, int DP, int NT>
 constexpr int kFwdOcc = DP * NT * (int)sizeof(T) > 512 ? (DP * NT * (int)sizeof(T) > 1024 ? 1 : 2) : 3;
 template <typename T, int DP, int NT>
+constexpr int kBwdRows = 32;  // rows of a backward tile
+template <typename T, int DP, int NT>
 constexpr int kBwdOcc = DP > 64 || (sizeof(T) == 4 && DP == 64 && NT == 1) ? 1 : (sizeof(T) == 2 && NT > 1 ? 3 : 2);
 
 template <typename T, int DP, int NT>
@@ -335,8 +337,10 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
   vbad = wave_any(vbad);
 
   const int32_t* list = a.list + (int64_t)unit * a.N * a.S + item.y;
-  const T* qp = static_cast<const T*>(a.q) + ((int64_t)b * a.N * a.H + (int64_t)hk * a.G) * D;
-  float* part = a.part + (int64_t)ug * a.N * a.S * a.G * D;
+  // rows are addressed as 32-bit row numbers times 32-bit row bytes
+  const uint8_t* qp = static_cast<const uint8_t*>(a.q) + ((int64_t)b * a.N * a.H + (int64_t)hk * a.G) * D * sizeof(T);
+  const uint32_t qbytes = (uint32_t)(a.H * D) * sizeof(T), pbytes = (uint32_t)(a.G * D) * 4;
+  uint8_t* part = reinterpret_cast<uint8_t*>(a.part + (int64_t)ug * a.N * a.S * a.G * D);
   float2* ml = a.ml + (int64_t)ug * a.N * a.S * a.G;
   const float sl2 = a.scale_log2;
 
@@ -350,9 +354,14 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
   int ent = entry_of(clamp(16 * w + c)), gh = head_of(clamp(16 * w + c));
   int entn = entry_of(clamp(16 * w + c + STEP));
   auto load_q = [&](F(&f)[NK], int e, int h) {
-    const T* p = qp + ((int64_t)(e >> 6) * a.H + h) * D;
+    const T* p = reinterpret_cast<const T*>(qp + (uint64_t)(uint32_t)(e >> 6) * qbytes + (uint32_t)(h * D) * sizeof(T));
+    if (D == DP) {
 #pragma unroll
-    for (int i = 0; i < NK; ++i) f[i] = 32 * i + 8 * g < D ? O::load(p + 32 * i + 8 * g) : O::zero();
+      for (int i = 0; i < NK; ++i) f[i] = O::load(p + 32 * i + 8 * g);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NK; ++i) f[i] = 32 * i + 8 * g < D ? O::load(p + 32 * i + 8 * g) : O::zero();
+    }
   };
   load_q(qf, ent, gh);
   for (int t0 = 16 * w; t0 < rows; t0 += STEP) {
@@ -369,30 +378,29 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
     for (int t = 0; t < NT; ++t) settle(s[t]);
     load_q(qf, entn, ghn);
     // keys of this row: up to its own (causal), up to the block's end
-    const int64_t qi = ent >> 6;
+    const int qi = ent >> 6;
     int lim = nk;
-    if (a.causal && qi - k0 + 1 < lim) lim = (int)(qi - k0 + 1);
+    if (a.causal && qi - (int)k0 + 1 < lim) lim = qi - (int)k0 + 1;
     const bool masked = wave_any(lim < 16 * NT);
+    if (masked) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        s[t][y] *= sl2;
-        if (masked) s[t][y] = 16 * t + 4 * g + y < lim ? s[t][y] : -INFINITY;
-      }
+        for (int y = 0; y < 4; ++y) s[t][y] = 16 * t + 4 * g + y < lim ? s[t][y] : -INFINITY;
+    }
     float m = -INFINITY;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int y = 0; y < 4; ++y) m = fmaxf(m, s[t][y]);
-    m = col_max(m);
-    const float mu = m == -INFINITY ? 0.0f : m;
+    m = col_max(m) * sl2;  // the scale is positive
+    const float mu = m == -INFINITY ? 0.0f : m - W::kBias;
     float p[2 * NP][4], l = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2 * NP; ++t)
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        p[t][y] = t < NT ? __builtin_amdgcn_exp2f(s[t < NT ? t : 0][y] - mu + W::kBias) : 0.0f;
+        p[t][y] = t < NT ? __builtin_amdgcn_exp2f(fmaf(s[t < NT ? t : 0][y], sl2, -mu)) : 0.0f;
         l += p[t][y];
       }
     l = col_sum(l);
@@ -434,8 +442,8 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
       }
     }
     if (t0 + c < rows) {
-      const int64_t at = (qi * a.S + (ent & 63)) * a.G + gh;
-      float* po = part + at * D;
+      const uint32_t pair = __umul24(qi, a.S) + (ent & 63);
+      float* po = reinterpret_cast<float*>(part + (uint64_t)pair * pbytes) + gh * D;
 #pragma unroll
       for (int y = 0; y < 4; ++y)
 #pragma unroll
@@ -447,7 +455,7 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
           else
             *reinterpret_cast<float4*>(po + d) = make_float4(acc[j][y], acc[j + 1][y], acc[j + 2][y], acc[j + 3][y]);
         }
-      if (g == 0) ml[at] = make_float2(m, l);
+      if (g == 0) ml[(int64_t)pair * a.G + gh] = make_float2(m, l);
     }
     ent = entn;
     entn = ent2;
@@ -474,37 +482,52 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Args a) {
   const int gh = (int)(rem - i * a.G), D = a.D;
   const int b = unit / a.Hkv, hk = unit % a.Hkv;
   const int32_t* row = row_of(a, unit, i);
+  const int64_t at = (((int64_t)ug * a.N + i) * a.S) * a.G + gh;  // slot s at + s * G
+  float2 x = make_float2(-INFINITY, 0.0f);
+  if (FWD && lane < a.S) x = a.ml[at + (int64_t)lane * a.G];  // not yet known to be written
   int e = lane < a.S ? listed(a, row, i, lane) : -1;
   for (int j = 0; j + 1 < a.S; ++j) {
     const int o = __builtin_amdgcn_readlane(e, j);
     if (j < lane && o == e) e = -1;
   }
   const uint64_t live = __ballot(e >= 0);
-  const int64_t at = (((int64_t)ug * a.N + i) * a.S) * a.G + gh;  // slot s at + s * G
-  float f = e >= 0 ? 1.0f : 0.0f, M = 0.0f, lt = 0.0f;
-  if constexpr (FWD) {
-    float2 x = make_float2(-INFINITY, 0.0f);
-    if (e >= 0) x = a.ml[at + (int64_t)lane * a.G];
-    M = x.x;
-#pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
-    const float mu = M == -INFINITY ? 0.0f : M;
-    f = e >= 0 ? __builtin_amdgcn_exp2f(x.x - mu) : 0.0f;
-    lt = e >= 0 ? f * x.y : 0.0f;
-#pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) lt += __shfl_xor(lt, k, 64);
-  }
+  // sixteen loads' worth of slots before their weights are needed
+  constexpr int SL = 64 / LP;  // slots at once
   const int d = 4 * (lane & (LP - 1));
+  const float* po = a.part + at * D + d;
+  const int64_t sstep = (int64_t)a.G * D;
+  float f = 1.0f, M = 0.0f, lt = 0.0f;
   float4 acc = make_float4(0, 0, 0, 0);
-  for (int s0 = 0; s0 < a.S; s0 += 64 / LP) {
-    const int s = s0 + lane / LP;
-    const float fs = __shfl(f, s & 63, 64);
-    if (s < a.S && (live >> s & 1) && d < D) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part + (at + (int64_t)s * a.G) * D + d);
-      acc.x += fs * x.x;
-      acc.y += fs * x.y;
-      acc.z += fs * x.z;
-      acc.w += fs * x.w;
+  for (int s0 = 0; s0 < a.S; s0 += 4 * SL) {
+    float4 v[4];
+    bool in[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int s = s0 + y * SL + lane / LP;
+      in[y] = s < a.S && (live >> s & 1) && d < D;
+      v[y] = make_float4(0, 0, 0, 0);
+      if (in[y]) v[y] = *reinterpret_cast<const float4*>(po + s * sstep);
+    }
+    if (FWD && s0 == 0) {
+      if (e < 0) x = make_float2(-INFINITY, 0.0f);
+      M = x.x;
+#pragma unroll
+      for (int k = 32; k >= 1; k >>= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
+      const float mu = M == -INFINITY ? 0.0f : M;
+      f = e >= 0 ? __builtin_amdgcn_exp2f(x.x - mu) : 0.0f;
+      lt = e >= 0 ? f * x.y : 0.0f;
+#pragma unroll
+      for (int k = 32; k >= 1; k >>= 1) lt += __shfl_xor(lt, k, 64);
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float fs = FWD ? __shfl(f, (s0 + y * SL + lane / LP) & 63, 64) : 1.0f;
+      if (in[y]) {
+        acc.x += fs * v[y].x;
+        acc.y += fs * v[y].y;
+        acc.z += fs * v[y].z;
+        acc.w += fs * v[y].w;
+      }
     }
   }
 #pragma unroll
@@ -517,8 +540,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Args a) {
   const int64_t orow = ((int64_t)b * a.N + i) * a.H + (int64_t)hk * a.G + gh;
   if (lane < LP && d < D) {
     T r[4];
-    float inv = 1.0f;
-    if (FWD) inv = live ? 1.0f / lt : 0.0f;
+    const float inv = FWD ? (live ? 1.0f / lt : 0.0f) : a.scale;
     if (FWD && !live) acc = make_float4(0, 0, 0, 0);
     r[0] = static_cast<T>(acc.x * inv);
     r[1] = static_cast<T>(acc.y * inv);
@@ -583,15 +605,15 @@ constexpr bool kScaled = __is_same(T, _Float16);
 // (f16's own) down to 2^-27 of the item's largest dS.
 template <typename T, int DP, int NT>
 struct BwdLds {
-  static constexpr int RT = 32;
+  static constexpr int RT = kBwdRows<T, DP, NT>;
   static constexpr int RS = DP * (int)sizeof(T) + 16;       // bytes of a staged row
   static constexpr int SS = RT * (int)sizeof(T) + 16;       // bytes of a key's dS
   static constexpr int kQ = 0;
   static constexpr int kG = RT * RS;
   static constexpr int kS = 2 * RT * RS;
   static constexpr int kSPlane = 16 * NT * SS;
-  static constexpr int kStat = kS + WeightPlanes<T>::N * kSPlane;  // lse, delta, pair [32]
-  static constexpr int kMax = kStat + 3 * RT * 4;                  // [NT] per-wave maxima
+  static constexpr int kStat = kS + WeightPlanes<T>::N * kSPlane;  // lse, delta, pair, last key [RT]
+  static constexpr int kMax = kStat + 4 * RT * 4;                  // [NT] per-wave maxima
   static constexpr int kFlag = kMax + NT * 4;                      // [2] tile flags, block flag
   static constexpr int kBytes = kFlag + 16;
 };
@@ -606,6 +628,7 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   constexpr int NK = DP / 32, ND = DP / 16, RT = L::RT;
   constexpr int TH = 64 * NT, CPR = DP / 8, NC = (RT * CPR + TH - 1) / TH;  // staged chunks per thread
   constexpr int JD = (ND + NT - 1) / NT, KC = (NT + 1) / 2;
+  static_assert(RT <= TH && RT % 32 == 0, "a thread per row of the tile");
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int x = xcd_row_order((int)blockIdx.x, (int)gridDim.x);
   const int ug = x / a.max_items, unit = a.unit0 + ug, slot_item = x % a.max_items;
@@ -613,12 +636,10 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   if (item.z < 0) return;
   const int rows = item.z * a.G;
   const int b = unit / a.Hkv, hk = unit % a.Hkv, D = a.D, blk = item.x;
-  const int64_t k0 = (int64_t)blk * a.BS, rs = (int64_t)a.Hkv * D;
-  const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.N * rs + hk * D;
-  const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.N * rs + hk * D;
-  const int64_t qbase = ((int64_t)b * a.N * a.H + (int64_t)hk * a.G) * D;
-  const T* qp = static_cast<const T*>(a.q) + qbase;
-  const T* gp = static_cast<const T*>(a.g) + qbase;
+  const int k0 = blk * a.BS;
+  const int64_t rs = (int64_t)a.Hkv * D;
+  const T* kp = static_cast<const T*>(a.k) + ((int64_t)b * a.N + k0) * rs + hk * D;
+  const T* vp = static_cast<const T*>(a.v) + ((int64_t)b * a.N + k0) * rs + hk * D;
   const int nk = (int)(a.N - k0 < 16 * NT ? a.N - k0 : 16 * NT);
 
   // this wave's keys as column operands, and K^T for its head_dim tiles
@@ -627,7 +648,7 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
     const bool ok = key < nk && 32 * i + 8 * g < D;
-    const int64_t at = (k0 + (key < nk ? key : 0)) * rs + (32 * i + 8 * g < D ? 32 * i + 8 * g : 0);
+    const int64_t at = (key < nk ? key : 0) * rs + (32 * i + 8 * g < D ? 32 * i + 8 * g : 0);
     kf[i] = O::load(kp + at);
     vf[i] = O::load(vp + at);
     if (!ok) kf[i] = vf[i] = O::zero();
@@ -642,7 +663,7 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
       for (int y = 0; y < 8; ++y) {
         const int kk = 32 * u + 16 * (y >> 2) + 4 * g + (y & 3);
         const bool ok = kk < nk && d < D;
-        e[y] = kp[(k0 + (kk < nk ? kk : 0)) * rs + (d < D ? d : 0)];
+        e[y] = kp[(kk < nk ? kk : 0) * rs + (d < D ? d : 0)];
         if (!ok) e[y] = static_cast<T>(0.0f);
       }
       kt[i][u] = __builtin_bit_cast(F, e);
@@ -658,19 +679,24 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   }
 
   const int32_t* list = a.list + (int64_t)unit * a.N * a.S + item.y;
-  float* part = a.part + (int64_t)ug * a.N * a.S * a.G * D;
-  const float* lse = a.lse_in + (int64_t)b * a.N * a.H + (int64_t)hk * a.G;
-  const float* dl = a.delta + (int64_t)b * a.N * a.H + (int64_t)hk * a.G;
+  const int64_t qbase = (int64_t)b * a.N * a.H + (int64_t)hk * a.G;
+  const uint8_t* qp = static_cast<const uint8_t*>(a.q) + qbase * D * sizeof(T);
+  const uint8_t* gp = static_cast<const uint8_t*>(a.g) + qbase * D * sizeof(T);
+  const uint32_t qbytes = (uint32_t)(a.H * D) * sizeof(T), pbytes = (uint32_t)(a.G * D) * 4;
+  uint8_t* part = reinterpret_cast<uint8_t*>(a.part + (int64_t)ug * a.N * a.S * a.G * D);
+  const float* lse = a.lse_in + qbase;
+  const float* dl = a.delta + qbase;
 
   // staging: chunk n of a thread is 8 elements of row (tid + n TH) / CPR; a
   // tile's pairs are read two tiles ahead, its rows one
   F sq[NC], sg[NC];
   int en[NC], est = 0;
-  int sflag = 0;
   float s_lse = INFINITY, s_dl = 0.0f;
-  int s_ent = 0;
+  int s_ent = 0, sown = 0;
   auto pair_of = [&](int rr) { return list[a.G == 1 ? rr : rr / a.G]; };
   auto head_of = [&](int rr) { return a.G == 1 ? 0 : rr % a.G; };
+  // a row inside the block has keys that it may not see
+  auto inside = [&](int e) { return a.causal && (e >> 6) - k0 < nk - 1; };
   auto pairs = [&](int r0) {
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -680,15 +706,16 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
     if (tid < RT) est = pair_of(r0 + tid < rows ? r0 + tid : rows - 1);
   };
   auto fetch = [&](int r0) {
-    sflag = 0;
+    sown = 0;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int ch = tid + n * TH, rr = r0 + ch / CPR, d = (ch % CPR) * 8;
       sq[n] = sg[n] = O::zero();
       if (ch < RT * CPR && rr < rows && d < D) {
-        const int64_t at = ((int64_t)(en[n] >> 6) * a.H + head_of(rr)) * D + d;
-        sq[n] = O::load(qp + at);
-        sg[n] = O::load(gp + at);
+        const uint64_t at = (uint64_t)(uint32_t)(en[n] >> 6) * qbytes + (uint32_t)(head_of(rr) * D + d) * sizeof(T);
+        sq[n] = O::load(reinterpret_cast<const T*>(qp + at));
+        sg[n] = O::load(reinterpret_cast<const T*>(gp + at));
+        sown |= inside(en[n]) << n;
       }
     }
     if (tid < RT) {
@@ -696,7 +723,7 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
       s_dl = 0.0f;
       s_ent = est;
       if (r0 + tid < rows) {
-        const int64_t at = (int64_t)(est >> 6) * a.H + head_of(r0 + tid);
+        const uint64_t at = (uint64_t)(uint32_t)(est >> 6) * (uint32_t)a.H + (uint32_t)head_of(r0 + tid);
         s_lse = lse[at];
         s_dl = dl[at];
       }
@@ -711,7 +738,9 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   float* st_lse = reinterpret_cast<float*>(lds + L::kStat);
   float* st_dl = st_lse + RT;
   int* st_ent = reinterpret_cast<int*>(st_dl + RT);
+  int* st_last = st_ent + RT;
   float* wmax = reinterpret_cast<float*>(lds + L::kMax);
+  const int kabs = key < nk ? k0 + key : INT32_MAX;  // a row sees it if this is at most its last key
 
   if (rows > 0) {
     pairs(0);
@@ -721,21 +750,22 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   int turn = 0;
   for (int r0 = 0; r0 < rows; r0 += RT, turn ^= 1) {
     __syncthreads();  // the last tile has been read
+    int sflag = 0;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int ch = tid + n * TH, row = ch / CPR, off = row * L::RS + (ch % CPR) * 8 * (int)sizeof(T);
       if (ch < RT * CPR) {
         *reinterpret_cast<F*>(lds + L::kQ + off) = sq[n];
         *reinterpret_cast<F*>(lds + L::kG + off) = sg[n];
-        if (a.causal && (O::bad(sq[n]) || O::bad(sg[n]))) sflag |= 2;
+        if ((sown >> n & 1) && (O::bad(sq[n]) || O::bad(sg[n]))) sflag |= 2;
       }
     }
     if (tid < RT) {
       st_lse[tid] = s_lse;
       st_dl[tid] = s_dl;
       st_ent[tid] = s_ent;
-      // a row inside the block has keys that it may not see
-      if (a.causal && r0 + tid < rows && (s_ent >> 6) - k0 < nk - 1) sflag |= 1;
+      st_last[tid] = r0 + tid >= rows ? -1 : (a.causal ? s_ent >> 6 : INT32_MAX - 1);
+      if (r0 + tid < rows && inside(s_ent)) sflag |= 1;
     }
     if (sflag) atomicOr(&flags[turn], sflag);
     if (tid == 0) flags[turn ^ 1] = 0;
@@ -747,131 +777,138 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
       pairs(r0 + 2 * RT);
     }
 
-    float p[2][4], ds[2][4];
-    bool ok[2][4];
+    int exs[RT / 32];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x4 s = f32x4{0, 0, 0, 0}, dp = f32x4{0, 0, 0, 0};
+    for (int h = 0; h < RT / 32; ++h) {  // 32 rows at a time
+      float p[2][4], ds[2][4];
+      bool ok[2][4];
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const uint8_t* at = lds + (16 * u + c) * L::RS + (32 * i + 8 * g) * (int)sizeof(T);
-        s = O::mma(O::load(reinterpret_cast<const T*>(at + L::kQ)), kf[i], s);
-        dp = O::mma(O::load(reinterpret_cast<const T*>(at + L::kG)), vf[i], dp);
-      }
-      settle(s);
-      settle(dp);
-      const float4 rl = *reinterpret_cast<const float4*>(st_lse + 16 * u + 4 * g);
-      const float4 rd = *reinterpret_cast<const float4*>(st_dl + 16 * u + 4 * g);
-      const int4 rq = *reinterpret_cast<const int4*>(st_ent + 16 * u + 4 * g);
-      const float le[4] = {rl.x, rl.y, rl.z, rl.w}, de[4] = {rd.x, rd.y, rd.z, rd.w};
-      const int qi[4] = {rq.x >> 6, rq.y >> 6, rq.z >> 6, rq.w >> 6};
+      for (int u = 0; u < 2; ++u) {
+        const int ru = 32 * h + 16 * u;
+        f32x4 s = f32x4{0, 0, 0, 0}, dp = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        ok[u][y] = key < nk && (!a.causal || k0 + key <= qi[y]) && r0 + 16 * u + 4 * g + y < rows;
-        const float pr = __builtin_amdgcn_exp2f(s[y] * sl2 - le[y]);
-        ds[u][y] = ok[u][y] ? pr * (dp[y] - de[y]) * a.scale : 0.0f;
-        p[u][y] = ok[u][y] ? pr * __builtin_amdgcn_exp2f(W::kBias) : 0.0f;
-      }
-    }
-    if constexpr (kScaled<T>) {
-      float mx = 0.0f;
+        for (int i = 0; i < NK; ++i) {
+          const uint8_t* at = lds + (ru + c) * L::RS + (32 * i + 8 * g) * (int)sizeof(T);
+          s = O::mma(O::load(reinterpret_cast<const T*>(at + L::kQ)), kf[i], s);
+          dp = O::mma(O::load(reinterpret_cast<const T*>(at + L::kG)), vf[i], dp);
+        }
+        settle(s);
+        settle(dp);
+        const float4 rl = *reinterpret_cast<const float4*>(st_lse + ru + 4 * g);
+        const float4 rd = *reinterpret_cast<const float4*>(st_dl + ru + 4 * g);
+        const int4 rq = *reinterpret_cast<const int4*>(st_last + ru + 4 * g);
+        const float le[4] = {rl.x, rl.y, rl.z, rl.w}, de[4] = {rd.x, rd.y, rd.z, rd.w};
+        const int last[4] = {rq.x, rq.y, rq.z, rq.w};
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) mx = fmaxf(mx, fabsf(ds[u][y]));
-#pragma unroll
-      for (int k = 32; k >= 1; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
-      if (lane == 0) wmax[w] = mx;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NT; ++i) mx = fmaxf(mx, wmax[i]);
-      if (mx > 0.0f) {
-        const int e = min(14 - __builtin_amdgcn_frexp_expf(mx), 100);
-        if (e < ex) {
-          const float f = ldexpf(1.0f, e - ex);
-#pragma unroll
-          for (int j = 0; j < ND; ++j)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) dk[j][y] *= f;
-          ex = e;
+        for (int y = 0; y < 4; ++y) {
+          ok[u][y] = kabs <= last[y];
+          const float pr = __builtin_amdgcn_exp2f(fmaf(s[y], sl2, -le[y]));
+          ds[u][y] = ok[u][y] ? pr * (dp[y] - de[y]) : 0.0f;  // the scale is applied to the results
+          p[u][y] = ok[u][y] ? pr * __builtin_amdgcn_exp2f(W::kBias) : 0.0f;
         }
       }
-      const float f = ldexpf(1.0f, ex);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) ds[u][y] *= f;
-    }
-    W pw, sw;
-    pw.set(p[0], p[1]);
-    sw.set(ds[0], ds[1]);
-    if (__builtin_expect(slow, 0)) {
-      // a row's infinity or NaN must not reach keys that it does not see
-      for (int rr = 0; rr < RT; ++rr) {
-        float pk = 0.0f, dk1 = 0.0f;
-        int okk = 0;
+      if constexpr (kScaled<T>) {
+        float mx = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (u == rr >> 4 && y == (rr & 3)) pk = p[u][y], dk1 = ds[u][y], okk = ok[u][y];
-        const int src = c + 16 * ((rr & 15) >> 2);
-        pk = __shfl(pk, src, 64);
-        dk1 = __shfl(dk1, src, 64);
-        okk = __shfl(okk, src, 64);
-        const T* qr = reinterpret_cast<const T*>(lds + L::kQ + rr * L::RS);
-        const T* gr = reinterpret_cast<const T*>(lds + L::kG + rr * L::RS);
-        if (okk)
+          for (int y = 0; y < 4; ++y) mx = fmaxf(mx, fabsf(ds[u][y]));
 #pragma unroll
-          for (int j = 0; j < ND; ++j)
+        for (int k = 32; k >= 1; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
+        if (h) __syncthreads();  // the last maxima have been read
+        if (lane == 0) wmax[w] = mx;
+        __syncthreads();
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              dv[j][y] += pk * (float)gr[16 * j + 4 * g + y];
-              dk[j][y] += dk1 * (float)qr[16 * j + 4 * g + y];
-            }
-      }
-    } else {
+        for (int i = 0; i < NT; ++i) mx = fmaxf(mx, wmax[i]);
+        if (mx > 0.0f) {
+          const int e = min(14 - __builtin_amdgcn_frexp_expf(mx), 100);
+          if (e < ex) {
+            const float f = ldexpf(1.0f, e - ex);
 #pragma unroll
-      for (int j = 0; j < ND; ++j) {
-        F gt, qt;
-        if constexpr (sizeof(T) == 2) {
-          const uint8_t* at = lds + (4 * g + (c >> 2)) * L::RS + (16 * j + 4 * (c & 3)) * 2;
-          const uint2 g0 = tr_read(at + L::kG), g1 = tr_read(at + L::kG + 16 * L::RS);
-          const uint2 q0 = tr_read(at + L::kQ), q1 = tr_read(at + L::kQ + 16 * L::RS);
-          gt = make_uint4(g0.x, g0.y, g1.x, g1.y);
-          qt = make_uint4(q0.x, q0.y, q1.x, q1.y);
-        } else {
+            for (int j = 0; j < ND; ++j)
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const uint8_t* at = lds + (16 * (y >> 2) + 4 * g + (y & 3)) * L::RS + (16 * j + c) * 4;
-            gt.v[y] = *reinterpret_cast<const float*>(at + L::kG);
-            qt.v[y] = *reinterpret_cast<const float*>(at + L::kQ);
+              for (int y = 0; y < 4; ++y) dk[j][y] *= f;
+            ex = e;
           }
         }
+        const float f = ldexpf(1.0f, ex);
 #pragma unroll
-        for (int pl = W::N - 1; pl >= 0; --pl) {
-          dv[j] = O::mma(gt, pw.w[pl], dv[j]);
-          dk[j] = O::mma(qt, sw.w[pl], dk[j]);
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) ds[u][y] *= f;
+      }
+      exs[h] = ex;
+      W pw, sw;
+      pw.set(p[0], p[1]);
+      sw.set(ds[0], ds[1]);
+      // dS [key][row] through LDS for dQ
+#pragma unroll
+      for (int pl = 0; pl < W::N; ++pl) {
+        uint8_t* at = lds + L::kS + pl * L::kSPlane + key * L::SS + (32 * h + 4 * g) * (int)sizeof(T);
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint2*>(at) = make_uint2(sw.w[pl].x, sw.w[pl].y);
+          *reinterpret_cast<uint2*>(at + 32) = make_uint2(sw.w[pl].z, sw.w[pl].w);
+        } else {
+          *reinterpret_cast<float4*>(at) = make_float4(ds[0][0], ds[0][1], ds[0][2], ds[0][3]);
+          *reinterpret_cast<float4*>(at + 64) = make_float4(ds[1][0], ds[1][1], ds[1][2], ds[1][3]);
         }
       }
-    }
-    // dS [key][row] through LDS for dQ
+      if (__builtin_expect(slow, 0)) {
+        // a row's infinity or NaN must not reach keys that it does not see
+        for (int rr = 0; rr < 32; ++rr) {
+          float pk = 0.0f, dk1 = 0.0f;
+          int okk = 0;
 #pragma unroll
-    for (int pl = 0; pl < W::N; ++pl) {
-      uint8_t* at = lds + L::kS + pl * L::kSPlane + key * L::SS + 4 * g * (int)sizeof(T);
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint2*>(at) = make_uint2(sw.w[pl].x, sw.w[pl].y);
-        *reinterpret_cast<uint2*>(at + 32) = make_uint2(sw.w[pl].z, sw.w[pl].w);
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (u == rr >> 4 && y == (rr & 3)) pk = p[u][y], dk1 = ds[u][y], okk = ok[u][y];
+          const int src = c + 16 * ((rr & 15) >> 2);
+          pk = __shfl(pk, src, 64);
+          dk1 = __shfl(dk1, src, 64);
+          okk = __shfl(okk, src, 64);
+          const T* qr = reinterpret_cast<const T*>(lds + L::kQ + (32 * h + rr) * L::RS);
+          const T* gr = reinterpret_cast<const T*>(lds + L::kG + (32 * h + rr) * L::RS);
+          if (okk)
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                dv[j][y] += pk * (float)gr[16 * j + 4 * g + y];
+                dk[j][y] += dk1 * (float)qr[16 * j + 4 * g + y];
+              }
+        }
       } else {
-        *reinterpret_cast<float4*>(at) = make_float4(ds[0][0], ds[0][1], ds[0][2], ds[0][3]);
-        *reinterpret_cast<float4*>(at + 64) = make_float4(ds[1][0], ds[1][1], ds[1][2], ds[1][3]);
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          F gt, qt;
+          if constexpr (sizeof(T) == 2) {
+            const uint8_t* at = lds + (32 * h + 4 * g + (c >> 2)) * L::RS + (16 * j + 4 * (c & 3)) * 2;
+            const uint2 g0 = tr_read(at + L::kG), g1 = tr_read(at + L::kG + 16 * L::RS);
+            const uint2 q0 = tr_read(at + L::kQ), q1 = tr_read(at + L::kQ + 16 * L::RS);
+            gt = make_uint4(g0.x, g0.y, g1.x, g1.y);
+            qt = make_uint4(q0.x, q0.y, q1.x, q1.y);
+          } else {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const uint8_t* at = lds + (32 * h + 16 * (y >> 2) + 4 * g + (y & 3)) * L::RS + (16 * j + c) * 4;
+              gt.v[y] = *reinterpret_cast<const float*>(at + L::kG);
+              qt.v[y] = *reinterpret_cast<const float*>(at + L::kQ);
+            }
+          }
+#pragma unroll
+          for (int pl = W::N - 1; pl >= 0; --pl) {
+            dv[j] = O::mma(gt, pw.w[pl], dv[j]);
+            dk[j] = O::mma(qt, sw.w[pl], dk[j]);
+          }
+        }
       }
     }
     __syncthreads();
-    const float back = kScaled<T> ? ldexpf(1.0f, -ex) : 1.0f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < RT / 16; ++u) {
       const int rr = r0 + 16 * u + c;
+      const float back = kScaled<T> ? ldexpf(1.0f, -exs[u / 2]) : 1.0f;
       f32x4 dq[JD];
 #pragma unroll
       for (int i = 0; i < JD; ++i) dq[i] = f32x4{0, 0, 0, 0};
@@ -908,19 +945,19 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
 #pragma unroll
           for (int pl = W::N - 1; pl >= 0; --pl)
             d1 += (float)*reinterpret_cast<const T*>(lds + L::kS + pl * L::kSPlane + kk * L::SS + (16 * u + c) * (int)sizeof(T));
-          if (k0 + kk > st_ent[16 * u + c] >> 6) continue;
+          if (k0 + kk > st_last[16 * u + c]) continue;
 #pragma unroll
           for (int i = 0; i < JD; ++i)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const int d = 16 * (w + NT * i) + 4 * g + y;
-              if (d < D) dq[i][y] += d1 * (float)kp[(k0 + kk) * rs + d];
+              if (d < D) dq[i][y] += d1 * (float)kp[kk * rs + d];
             }
         }
       }
       if (rr < rows) {
-        const int e = st_ent[16 * u + c], gh = head_of(rr);
-        float* po = part + (((int64_t)(e >> 6) * a.S + (e & 63)) * a.G + gh) * D;
+        const int e = st_ent[16 * u + c];
+        float* po = reinterpret_cast<float*>(part + (uint64_t)(__umul24(e >> 6, a.S) + (e & 63)) * pbytes) + head_of(rr) * D;
 #pragma unroll
         for (int i = 0; i < JD; ++i) {
           const int d = 16 * (w + NT * i) + 4 * g;
@@ -933,7 +970,7 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   }
   // dK, dV: the only item of its block stores them, others leave parts
   const bool single = a.blk_items[(int64_t)unit * a.nb + blk].y == 1;
-  const float fv = __builtin_amdgcn_exp2f(-W::kBias), fk = kScaled<T> ? ldexpf(1.0f, -ex) : 1.0f;
+  const float fv = __builtin_amdgcn_exp2f(-W::kBias), fk = (kScaled<T> ? ldexpf(1.0f, -ex) : 1.0f) * a.scale;
   if (key >= nk) return;
 #pragma unroll
   for (int j = 0; j < ND; ++j) {
@@ -946,7 +983,7 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
         k4[y] = static_cast<T>(dk[j][y] * fk);
         v4[y] = static_cast<T>(dv[j][y] * fv);
       }
-      const int64_t at = (int64_t)b * a.N * rs + (k0 + key) * rs + hk * D + d;
+      const int64_t at = ((int64_t)b * a.N + k0 + key) * rs + hk * D + d;
       T* ok = static_cast<T*>(a.dk) + at;
       T* ov = static_cast<T*>(a.dv) + at;
       if constexpr (sizeof(T) == 2) {
