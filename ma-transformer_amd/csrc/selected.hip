@@ -16,7 +16,7 @@ struct Layout {
   Args a;
   int64_t units;
   int64_t group;  // units per launch
-  size_t counts, offs, list, items, blk_items, part, ml, delta, part_kv, total;
+  size_t counts, offs, list, items, blk_items, part, ml, delta, part_kv, unread, total;
 };
 
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -72,6 +72,7 @@ Layout layout(const ma_select_desc* d, bool backward) {
   if (backward) {
     l.delta = take((size_t)d->batch * a.N * a.H * sizeof(float));
     l.part_kv = take(g * a.max_items * 2 * a.BS * a.D * sizeof(float));
+    l.unread = take(a.D * sizeof(float));
   } else {
     l.ml = take(g * pairs * sizeof(float2));
   }
@@ -93,6 +94,7 @@ int place(Layout& l, const ma_select_desc* d, void* ws, size_t bytes, const char
   a.ml = reinterpret_cast<float2*>(p + l.ml);
   a.delta = reinterpret_cast<float*>(p + l.delta);
   a.part_kv = reinterpret_cast<float*>(p + l.part_kv);
+  a.unread = reinterpret_cast<float*>(p + l.unread);
   (void)d;
   return 0;
 }
@@ -139,32 +141,32 @@ void join(const Args& a, bool last, hipStream_t st) {
     ma_host::launch(last, join_kernel<T, 32, FWD>, grid, block, 0, st, a);
 }
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool FULL>
 int forward_dn(Layout l, hipStream_t st) {
   Args a = l.a;
   for (int64_t u = 0; u < l.units; u += l.group) {
     a.unit0 = (int32_t)u;
     a.units = (int32_t)std::min(l.group, l.units - u);
-    ma_host::launch(false, forward_kernel<T, DP, NT>, dim3((unsigned)(a.units * a.max_items)), dim3(64 * kFwdWaves), 0,
+    ma_host::launch(false, forward_kernel<T, DP, NT, FULL>, dim3((unsigned)(a.units * a.max_items)), dim3(64 * kFwdWaves), 0,
                     st, a);
     join<T, true>(a, u + l.group >= l.units, st);
   }
   return launched("ma_selected_forward");
 }
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool FULL>
 int backward_dn(Layout l, hipStream_t st) {
   Args a = l.a;
   constexpr size_t shm = BwdLds<T, DP, NT>::kBytes;
   if (shm > 48 * 1024 &&
-      ma_host::reserve_lds(reinterpret_cast<const void*>(&backward_kernel<T, DP, NT>), shm, st))
+      ma_host::reserve_lds(reinterpret_cast<const void*>(&backward_kernel<T, DP, NT, FULL>), shm, st))
     return 1;
   const int64_t rows = l.units / a.Hkv * a.N * a.H;
   ma_host::launch(false, delta_kernel<T>, dim3((unsigned)((rows * 8 + 255) / 256)), dim3(256), 0, st, a, rows);
   for (int64_t u = 0; u < l.units; u += l.group) {
     a.unit0 = (int32_t)u;
     a.units = (int32_t)std::min(l.group, l.units - u);
-    ma_host::launch(false, backward_kernel<T, DP, NT>, dim3((unsigned)(a.units * a.max_items)), dim3(64 * NT),
+    ma_host::launch(false, backward_kernel<T, DP, NT, FULL>, dim3((unsigned)(a.units * a.max_items)), dim3(64 * NT),
                     (uint32_t)shm, st, a);
     ma_host::launch(false, join_kv_kernel<T>, dim3((unsigned)(a.units * a.nb * kKvParts)), dim3(256), 0, st, a);
     join<T, false>(a, u + l.group >= l.units, st);
@@ -172,11 +174,17 @@ int backward_dn(Layout l, hipStream_t st) {
   return launched("ma_selected_backward");
 }
 
+template <typename T, int DP, bool BWD, bool FULL>
+int run_df(const Layout& l, hipStream_t st) {
+  if (l.a.BS == 16) return BWD ? backward_dn<T, DP, 1, FULL>(l, st) : forward_dn<T, DP, 1, FULL>(l, st);
+  if (l.a.BS == 32) return BWD ? backward_dn<T, DP, 2, FULL>(l, st) : forward_dn<T, DP, 2, FULL>(l, st);
+  return BWD ? backward_dn<T, DP, 4, FULL>(l, st) : forward_dn<T, DP, 4, FULL>(l, st);
+}
+
+// head_dim rounded up to DP; the kernels of exactly DP carry no tail.
 template <typename T, int DP, bool BWD>
 int run_d(const Layout& l, hipStream_t st) {
-  if (l.a.BS == 16) return BWD ? backward_dn<T, DP, 1>(l, st) : forward_dn<T, DP, 1>(l, st);
-  if (l.a.BS == 32) return BWD ? backward_dn<T, DP, 2>(l, st) : forward_dn<T, DP, 2>(l, st);
-  return BWD ? backward_dn<T, DP, 4>(l, st) : forward_dn<T, DP, 4>(l, st);
+  return l.a.D == DP ? run_df<T, DP, BWD, true>(l, st) : run_df<T, DP, BWD, false>(l, st);
 }
 
 template <typename T, bool BWD>

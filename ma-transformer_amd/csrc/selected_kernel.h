@@ -44,6 +44,7 @@ struct Args {
   float2* ml;        // [N][S][G]
   float* delta;      // [B][N][H]
   float* part_kv;    // group's items: [max_items][2][BS][D]
+  float* unread;     // [D] written and never read
   int64_t N;
   int32_t H, Hkv, G, D, S, BS, nb, causal;
   int32_t chunks, words, max_items, cap;  // cap: pairs per item
@@ -58,7 +59,7 @@ struct Args {
 // and ranks are population counts, so the lists come out in query order
 // whatever order the threads run in.
 
-constexpr int kListThreads = 256;
+constexpr int kListThreads = 1024;
 constexpr int kScanThreads = 1024;
 
 // Entry j of a query's list: its block, or -1 where it is skipped.
@@ -287,20 +288,21 @@ constexpr int kBwdRows = 32;  // rows of a backward tile
 template <typename T, int DP, int NT>
 constexpr int kBwdOcc = DP > 64 || (sizeof(T) == 4 && DP == 64 && NT == 1) ? 1 : (sizeof(T) == 2 && NT > 1 ? 3 : 2);
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool FULL>
 __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_kernel(Args a) {
   using O = Op<T>;
   using F = typename O::F;
   using W = WeightPlanes<T>;
   using VR = ValueRows<T, DP>;
   constexpr int NK = DP / 32, NP = (NT + 1) / 2, VPL = VR::VPL;
+  __shared__ __attribute__((aligned(16))) float tile_o[kFwdWaves][16][DP + 4];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int x = xcd_row_order((int)blockIdx.x, (int)gridDim.x);
+  const int x = (int)blockIdx.x;
   const int ug = x / a.max_items, unit = a.unit0 + ug;
   const int4 item = a.items[(int64_t)unit * a.max_items + x % a.max_items];
   const int rows = item.z * a.G;
   if (rows <= 16 * w) return;
-  const int b = unit / a.Hkv, hk = unit % a.Hkv, D = a.D, blk = item.x;
+  const int b = unit / a.Hkv, hk = unit % a.Hkv, D = FULL ? DP : a.D, blk = item.x;
   const int64_t k0 = (int64_t)blk * a.BS, rs = (int64_t)a.Hkv * D;
   const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.N * rs + hk * D;
   const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.N * rs + hk * D;
@@ -344,7 +346,9 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
   float2* ml = a.ml + (int64_t)ug * a.N * a.S * a.G;
   const float sl2 = a.scale_log2;
 
-  // a row past the end repeats the last one and is not stored
+  // a row past the end repeats the last one and stores the same values to the
+  // same place: memory operations under a branch would make the wait for the
+  // next queries one for these stores too (230 -> 150 us)
   auto entry_of = [&](int r) { return list[(a.G == 1 ? r : r / a.G)]; };
   auto head_of = [&](int r) { return a.G == 1 ? 0 : r % a.G; };
   auto clamp = [&](int r) { return r < rows ? r : rows - 1; };
@@ -355,16 +359,11 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
   int entn = entry_of(clamp(16 * w + c + STEP));
   auto load_q = [&](F(&f)[NK], int e, int h) {
     const T* p = reinterpret_cast<const T*>(qp + (uint64_t)(uint32_t)(e >> 6) * qbytes + (uint32_t)(h * D) * sizeof(T));
-    if (D == DP) {
 #pragma unroll
-      for (int i = 0; i < NK; ++i) f[i] = O::load(p + 32 * i + 8 * g);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NK; ++i) f[i] = 32 * i + 8 * g < D ? O::load(p + 32 * i + 8 * g) : O::zero();
-    }
+    for (int i = 0; i < NK; ++i) f[i] = FULL || 32 * i + 8 * g < D ? O::load(p + 32 * i + 8 * g) : O::zero();
   };
   load_q(qf, ent, gh);
-  for (int t0 = 16 * w; t0 < rows; t0 += STEP) {
+  auto tile = [&](int t0) {
     const int ghn = head_of(clamp(t0 + STEP + c));
     const int ent2 = entry_of(clamp(t0 + 2 * STEP + c));
     f32x4 s[NT];
@@ -441,26 +440,43 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
           }
       }
     }
-    if (t0 + c < rows) {
-      const uint32_t pair = __umul24(qi, a.S) + (ent & 63);
-      float* po = reinterpret_cast<float*>(part + (uint64_t)pair * pbytes) + gh * D;
+    // through LDS, so that a store writes whole rows
+    const uint32_t pair = __umul24(qi, a.S) + (ent & 63);
+    float* mine = &tile_o[w][c][0];
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
+    for (int y = 0; y < 4; ++y)
 #pragma unroll
-        for (int j = 0; j < VPL; j += VR::CH) {
-          const int d = VR::element(g, y, j);
-          if (d >= D) continue;
-          if constexpr (VPL == 2)
-            *reinterpret_cast<float2*>(po + d) = make_float2(acc[0][y], acc[1][y]);
-          else
-            *reinterpret_cast<float4*>(po + d) = make_float4(acc[j][y], acc[j + 1][y], acc[j + 2][y], acc[j + 3][y]);
-        }
-      if (g == 0) ml[(int64_t)pair * a.G + gh] = make_float2(m, l);
+      for (int j = 0; j < VPL; j += VR::CH) {
+        const int d = VR::element(g, y, j);
+        if constexpr (VPL == 2)
+          *reinterpret_cast<float2*>(mine + d) = make_float2(acc[0][y], acc[1][y]);
+        else
+          *reinterpret_cast<float4*>(mine + d) = make_float4(acc[j][y], acc[j + 1][y], acc[j + 2][y], acc[j + 3][y]);
+      }
+    ml[(int64_t)pair * a.G + gh] = make_float2(m, l);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int CPR = DP / 4, RPI = 64 / CPR;  // 16-byte chunks of a row, rows of a store
+#pragma unroll
+    for (int it = 0; it < 16 / RPI; ++it) {
+      const int row = it * RPI + lane / CPR, d = (lane % CPR) * 4;
+      const uint32_t pr = __shfl((int)pair, row, 64);
+      const int gr = a.G == 1 ? 0 : __shfl(gh, row, 64);
+      float* po = reinterpret_cast<float*>(part + (uint64_t)pr * pbytes) + gr * D + d;
+      if (FULL || d < D)
+        __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(&tile_o[w][row][d]), reinterpret_cast<f32x4*>(po));
     }
+    __builtin_amdgcn_wave_barrier();
     ent = entn;
     entn = ent2;
     gh = ghn;
-  }
+  };
+  // the first tile stands before the loop, which is then entered as it repeats:
+  // with the next queries under way and this tile's stores behind them.  Where
+  // the two ways in differ the compiler waits for the lesser count, and with it
+  // for stores.
+  tile(16 * w);
+  for (int t0 = 16 * w + STEP; t0 < rows; t0 += STEP) tile(t0);
 }
 
 // ---------------------------------------------------------------- joining a query's slots
@@ -499,14 +515,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Args a) {
   float f = 1.0f, M = 0.0f, lt = 0.0f;
   float4 acc = make_float4(0, 0, 0, 0);
   for (int s0 = 0; s0 < a.S; s0 += 4 * SL) {
-    float4 v[4];
+    f32x4 v[4];
     bool in[4];
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int s = s0 + y * SL + lane / LP;
       in[y] = s < a.S && (live >> s & 1) && d < D;
-      v[y] = make_float4(0, 0, 0, 0);
-      if (in[y]) v[y] = *reinterpret_cast<const float4*>(po + s * sstep);
+      v[y] = f32x4{0, 0, 0, 0};
+      if (in[y]) v[y] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(po + s * sstep));
     }
     if (FWD && s0 == 0) {
       if (e < 0) x = make_float2(-INFINITY, 0.0f);
@@ -523,10 +539,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(Args a) {
     for (int y = 0; y < 4; ++y) {
       const float fs = FWD ? __shfl(f, (s0 + y * SL + lane / LP) & 63, 64) : 1.0f;
       if (in[y]) {
-        acc.x += fs * v[y].x;
-        acc.y += fs * v[y].y;
-        acc.z += fs * v[y].z;
-        acc.w += fs * v[y].w;
+        acc.x += fs * v[y][0];
+        acc.y += fs * v[y][1];
+        acc.z += fs * v[y][2];
+        acc.w += fs * v[y][3];
       }
     }
   }
@@ -618,7 +634,7 @@ struct BwdLds {
   static constexpr int kBytes = kFlag + 16;
 };
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool FULL>
 __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   using O = Op<T>;
@@ -630,12 +646,12 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   constexpr int JD = (ND + NT - 1) / NT, KC = (NT + 1) / 2;
   static_assert(RT <= TH && RT % 32 == 0, "a thread per row of the tile");
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int x = xcd_row_order((int)blockIdx.x, (int)gridDim.x);
+  const int x = (int)blockIdx.x;
   const int ug = x / a.max_items, unit = a.unit0 + ug, slot_item = x % a.max_items;
   const int4 item = a.items[(int64_t)unit * a.max_items + slot_item];
   if (item.z < 0) return;
   const int rows = item.z * a.G;
-  const int b = unit / a.Hkv, hk = unit % a.Hkv, D = a.D, blk = item.x;
+  const int b = unit / a.Hkv, hk = unit % a.Hkv, D = FULL ? DP : a.D, blk = item.x;
   const int k0 = blk * a.BS;
   const int64_t rs = (int64_t)a.Hkv * D;
   const T* kp = static_cast<const T*>(a.k) + ((int64_t)b * a.N + k0) * rs + hk * D;
@@ -691,7 +707,7 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   // tile's pairs are read two tiles ahead, its rows one
   F sq[NC], sg[NC];
   int en[NC], est = 0;
-  float s_lse = INFINITY, s_dl = 0.0f;
+  float s_lse = 0.0f, s_dl = 0.0f;
   int s_ent = 0, sown = 0;
   auto pair_of = [&](int rr) { return list[a.G == 1 ? rr : rr / a.G]; };
   auto head_of = [&](int rr) { return a.G == 1 ? 0 : rr % a.G; };
@@ -703,31 +719,29 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
       const int rr = r0 + (tid + n * TH) / CPR;
       en[n] = pair_of(rr < rows ? rr : rows - 1);
     }
-    if (tid < RT) est = pair_of(r0 + tid < rows ? r0 + tid : rows - 1);
+    const int rt = r0 + (tid & (RT - 1));
+    est = pair_of(rt < rows ? rt : rows - 1);
   };
+  // no load and no store of the loop stands under a branch (rows past the end
+  // load the last row, and store their dQ to a row that nothing reads): the
+  // wait for the next tile's rows would otherwise be one for this tile's
+  // stores too
   auto fetch = [&](int r0) {
     sown = 0;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int ch = tid + n * TH, rr = r0 + ch / CPR, d = (ch % CPR) * 8;
-      sq[n] = sg[n] = O::zero();
-      if (ch < RT * CPR && rr < rows && d < D) {
-        const uint64_t at = (uint64_t)(uint32_t)(en[n] >> 6) * qbytes + (uint32_t)(head_of(rr) * D + d) * sizeof(T);
-        sq[n] = O::load(reinterpret_cast<const T*>(qp + at));
-        sg[n] = O::load(reinterpret_cast<const T*>(gp + at));
-        sown |= inside(en[n]) << n;
-      }
+      const int hd = head_of(rr < rows ? rr : rows - 1) * D + (FULL || d < D ? d : 0);
+      const uint64_t at = (uint64_t)(uint32_t)(en[n] >> 6) * qbytes + (uint32_t)hd * sizeof(T);
+      sq[n] = O::load(reinterpret_cast<const T*>(qp + at));
+      sg[n] = O::load(reinterpret_cast<const T*>(gp + at));
+      sown |= inside(en[n]) << n;
     }
-    if (tid < RT) {
-      s_lse = INFINITY;  // a row past the end has no weight
-      s_dl = 0.0f;
-      s_ent = est;
-      if (r0 + tid < rows) {
-        const uint64_t at = (uint64_t)(uint32_t)(est >> 6) * (uint32_t)a.H + (uint32_t)head_of(r0 + tid);
-        s_lse = lse[at];
-        s_dl = dl[at];
-      }
-    }
+    const int rt = r0 + (tid & (RT - 1));
+    const uint64_t at = (uint64_t)(uint32_t)(est >> 6) * (uint32_t)a.H + (uint32_t)head_of(rt < rows ? rt : rows - 1);
+    s_lse = lse[at];
+    s_dl = dl[at];
+    s_ent = est;
   };
 
   f32x4 dv[ND], dk[ND];
@@ -754,6 +768,9 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int ch = tid + n * TH, row = ch / CPR, off = row * L::RS + (ch % CPR) * 8 * (int)sizeof(T);
+      if (r0 + RT > rows || !FULL) {  // zeros past the end and past head_dim
+        if (r0 + row >= rows || (ch % CPR) * 8 >= D) sq[n] = sg[n] = O::zero();
+      }
       if (ch < RT * CPR) {
         *reinterpret_cast<F*>(lds + L::kQ + off) = sq[n];
         *reinterpret_cast<F*>(lds + L::kG + off) = sg[n];
@@ -761,8 +778,8 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
       }
     }
     if (tid < RT) {
-      st_lse[tid] = s_lse;
-      st_dl[tid] = s_dl;
+      st_lse[tid] = r0 + tid < rows ? s_lse : INFINITY;  // a row past the end has no weight
+      st_dl[tid] = r0 + tid < rows ? s_dl : 0.0f;
       st_ent[tid] = s_ent;
       st_last[tid] = r0 + tid >= rows ? -1 : (a.causal ? s_ent >> 6 : INT32_MAX - 1);
       if (r0 + tid < rows && inside(s_ent)) sflag |= 1;
@@ -955,16 +972,16 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
             }
         }
       }
-      if (rr < rows) {
-        const int e = st_ent[16 * u + c];
-        float* po = reinterpret_cast<float*>(part + (uint64_t)(__umul24(e >> 6, a.S) + (e & 63)) * pbytes) + head_of(rr) * D;
+      const int e = st_ent[16 * u + c];
+      float* po = reinterpret_cast<float*>(part + (uint64_t)(__umul24(e >> 6, a.S) + (e & 63)) * pbytes) +
+                  head_of(rr < rows ? rr : rows - 1) * D;
+      po = rr < rows ? po : a.unread;
 #pragma unroll
-        for (int i = 0; i < JD; ++i) {
-          const int d = 16 * (w + NT * i) + 4 * g;
-          if (d < D)
-            *reinterpret_cast<float4*>(po + d) =
-                make_float4(dq[i][0] * back, dq[i][1] * back, dq[i][2] * back, dq[i][3] * back);
-        }
+      for (int i = 0; i < JD; ++i) {
+        const int d = 16 * (w + NT * i) + 4 * g;
+        if ((FULL && ND % NT == 0) || d < D)
+          __builtin_nontemporal_store(f32x4{dq[i][0] * back, dq[i][1] * back, dq[i][2] * back, dq[i][3] * back},
+                                      reinterpret_cast<f32x4*>(po + d));
       }
     }
   }
