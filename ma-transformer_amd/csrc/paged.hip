@@ -16,8 +16,8 @@ using ma_host::fail;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// A launch holds fewer than 2^32 threads; workgroups have at most 512.
-constexpr int64_t kMaxGrid = INT32_MAX / 512;
+// A launch holds fewer than 2^32 threads; workgroups have at most 1024.
+constexpr int64_t kMaxGrid = INT32_MAX / 1024;
 
 // What every call needs of a descriptor.
 int check(const ma_paged_desc* d, const char* who) {
@@ -54,7 +54,10 @@ int launched(const char* who) {
   return e == hipSuccess ? 0 : fail("%s: kernel launch failed: %s", who, hipGetErrorString(e));
 }
 
-// Workgroups a decode call splits its token range over.  Units = (stream, kv
+// Workgroups a decode call splits its token range over: from 2048 keys on, as
+// many as fill the card (1024, four a CU).  A split costs the second launch:
+// 1024 listed keys of 32 x 4 heads take 12.4 us unsplit, 11.4 + 4.0 in two
+// parts; 65536 keys of 8 heads 24-26 us in 64 to 256 parts.  Units = (stream, kv
 // head, 16 query heads).
 int64_t decode_splits(const ma_paged_desc* d) {
   const int64_t G = d->num_heads / d->num_kv_heads;
@@ -64,7 +67,7 @@ int64_t decode_splits(const ma_paged_desc* d) {
     keys = std::min(keys, d->num_selected * d->page_size);
   else if (d->left >= 0 && d->left < keys)
     keys = std::min(keys, d->left + 32 + std::min(std::max<int64_t>(d->num_global, 0), keys));
-  const int64_t most = std::max<int64_t>(1, keys / 512);
+  const int64_t most = std::max<int64_t>(1, keys / 1024);
   const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(units, 1));
   return std::min({most, want, (int64_t)kMaxSplit});
 }
@@ -96,8 +99,13 @@ int decode_t(const ma_paged_desc* d, const DecodeArgs& a, hipStream_t st) {
     decode_dp<T, 64>(a, grid, join, st);
   else
     decode_dp<T, 128>(a, grid, join, st);
-  if (join)
-    ma_host::launch(true, decode_join_kernel<T>, dim3((unsigned)(d->batch * a.H)), dim3(kJoinThreads), 0, st, a);
+  const dim3 rows((unsigned)(d->batch * a.H)), threads(kJoinThreads);
+  if (join && a.D <= 32)
+    ma_host::launch(true, decode_join_kernel<T, 32>, rows, threads, 0, st, a);
+  else if (join && a.D <= 64)
+    ma_host::launch(true, decode_join_kernel<T, 64>, rows, threads, 0, st, a);
+  else if (join)
+    ma_host::launch(true, decode_join_kernel<T, 128>, rows, threads, 0, st, a);
   return launched("ma_paged_decode");
 }
 

@@ -19,8 +19,8 @@ using namespace ma_dev;
 // same way whoever computes it.  The angles of a tile of tokens are computed
 // once into LDS and serve every query and key head.
 //
-// One workgroup takes one page's worth of positions of one stream, so that
-// with page sums it owns the page: after its stores it reads the page's stored
+// One workgroup takes one page's worth of positions of one stream, so that with
+// page sums it owns the page: after its stores it reads the page's stored
 // keys [0, end) back (cache-hot) and adds them in slot order classes.  The sum
 // depends on the page's contents alone, not on the calls that filled it: a
 // stream that is set back and appended to again needs no correction.
@@ -46,7 +46,8 @@ struct AppendArgs {
   int32_t wgs;      // workgroups per stream
 };
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 512;
+constexpr int kSumParts = kAppendThreads / 32;  // slot classes of a page sum
 constexpr int kAppendTile = 16;  // tokens whose angles are in LDS at once
 
 // Eight elements as float32 values or raw bits.
@@ -126,6 +127,7 @@ __device__ __forceinline__ void rotate_unit(const T* src, T* dst, int u, int R, 
 template <typename T>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int32_t s_slot[kAppendTile];
   double2* cs = reinterpret_cast<double2*>(lds);  // [kAppendTile][R / 2]
   const int tid = threadIdx.x;
   const int64_t b = blockIdx.x / (uint32_t)a.wgs;
@@ -147,52 +149,67 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
   T* ck = static_cast<T*>(a.ck);
   T* cv = static_cast<T*>(a.cv);
   T* qo = static_cast<T*>(a.qo);
+  const int nr = nk + nq;
+  const int tv = tid / nv, uv = tid - tv * nv, sv = kAppendThreads / nv;
+  const int tr = tid / nr, ur = tid - tr * nr, sr = kAppendThreads / nr;
+  const uint32_t kvrow = (uint32_t)(a.Hkv * D);
   for (int64_t t0 = p0; t0 < p1; t0 += kAppendTile) {
     const int nt = (int)(p1 - t0 < kAppendTile ? p1 - t0 : kAppendTile);
+    __syncthreads();  // the last tile's angles and slots have been read
+    if (tid < nt) {
+      // where the token is stored; -1: behind the count, the table or the cache
+      const int64_t pos = t0 + tid, l = pos / a.page;
+      int32_t slot = -1;
+      if (pos - s0 < cnt && l < a.width) {
+        const int32_t ph = a.table[b * a.width + l];
+        if (ph >= 0 && ph < a.pages) slot = ph * a.page + (int32_t)(pos - l * a.page);
+      }
+      s_slot[tid] = slot;
+    }
     if (half) {
-      __syncthreads();  // the last tile's angles have been read
       for (int e = tid; e < nt * half; e += kAppendThreads) {
         const int t = e / half, j = e - t * half;
         double s, c;
         sincos((double)(t0 + t) * a.freq[j], &s, &c);
         cs[t * half + j] = make_double2(c, s);
       }
-      __syncthreads();
     }
-    const int per = nk + nv + nq;
-    for (int e = tid; e < nt * per; e += kAppendThreads) {
-      const int t = e / per;
-      int u = e - t * per;
-      const int64_t pos = t0 + t, row = b * a.n + (pos - s0);
-      if (u >= nk + nv) {
-        u -= nk + nv;
-        const int h = u / upr;
-        const int64_t o = (row * a.H + h) * D;
-        rotate_unit<T>(qin + o, qo + o, u - h * upr, R, a.inter, cs + t * half);
-        continue;
+    __syncthreads();
+    const uint32_t row0 = (uint32_t)(t0 - s0);
+    // values: chunk u of token t, a step of kAppendThreads chunks at a time (the
+    // heads' values are one run of elements)
+    for (int t = tv, u = uv; t < nt; t += sv, u += kAppendThreads - sv * nv) {
+      if (u >= nv) {
+        u -= nv;
+        if (++t >= nt) break;
       }
-      if (pos - s0 >= cnt) continue;
-      const int64_t l = pos / a.page;
-      if (l >= a.width) continue;
-      const int32_t ph = a.table[b * a.width + l];
-      if (ph < 0 || ph >= a.pages) continue;
-      const int64_t slot = (int64_t)ph * a.page + (pos - l * a.page);
-      if (u < nk) {
-        const int h = u / upr;
-        rotate_unit<T>(kin + (row * a.Hkv + h) * D, ck + (slot * a.Hkv + h) * D, u - h * upr, R, a.inter,
-                       cs + t * half);
-      } else {
-        u -= nk;  // a token's values are one run of Hkv * D elements
-        Vec8<T> x;
-        x.load(vin + row * a.Hkv * D + 8 * u);
-        x.store(cv + slot * a.Hkv * D + 8 * u);
+      const int32_t slot = s_slot[t];
+      const uint64_t row = (uint64_t)b * (uint32_t)a.n + (row0 + t);
+      Vec8<T> x;
+      x.load(vin + row * kvrow + 8 * u);
+      if (slot >= 0) x.store(cv + (uint64_t)(uint32_t)slot * kvrow + 8 * u);
+    }
+    // keys and queries, which differ in their addresses alone: lanes of one wave
+    // take the same path
+    for (int t = tr, u = ur; t < nt; t += sr, u += kAppendThreads - sr * nr) {
+      if (u >= nr) {
+        u -= nr;
+        if (++t >= nt) break;
       }
+      const int32_t slot = s_slot[t];
+      const uint64_t row = (uint64_t)b * (uint32_t)a.n + (row0 + t);
+      const bool isq = u >= nk;
+      if (!isq && slot < 0) continue;
+      const uint32_t v = (uint32_t)(isq ? u - nk : u), h = v / (uint32_t)upr;
+      const uint64_t qo_at = row * (uint32_t)(a.H * D) + h * D, ki = row * kvrow + h * D;
+      const T* src = isq ? qin + qo_at : kin + ki;
+      T* dst = isq ? qo + qo_at : ck + (uint64_t)(uint32_t)slot * kvrow + h * D;
+      rotate_unit<T>(src, dst, (int)(v - h * upr), R, a.inter, cs + t * half);
     }
   }
   if (!a.sums) return;
   // the page's stored keys, back from the cache: thread (r, c) adds every
-  // (threads per chunk)-th slot of 8 elements, and the r parts are joined in
-  // order
+  // kSumParts-th slot of 8 elements, and the parts are joined in order
   const int64_t last = p1 < s0 + cnt ? p1 : s0 + cnt;
   const int64_t l = p0 / a.page;
   if (last <= p0 || l >= a.width) return;
@@ -200,7 +217,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
   if (ph < 0 || ph >= a.pages) return;
   const int end = (int)(last - l * a.page);
   __syncthreads();  // every store of this workgroup is visible to it; the angles are free
-  float* part = reinterpret_cast<float*>(lds);  // [8 parts][32 chunks][8]
+  float* part = reinterpret_cast<float*>(lds);  // [kSumParts][32 chunks][8]
   const int chunks = a.Hkv * (D >> 3);
   const int r = tid >> 5, c0 = tid & 31;
   for (int cb = 0; cb < chunks; cb += 32) {
@@ -209,7 +226,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
     if (c < chunks) {
       const T* p = ck + (int64_t)ph * a.page * a.Hkv * D + 8 * c;
 #pragma unroll 4
-      for (int s = r; s < end; s += 8) {
+      for (int s = r; s < end; s += kSumParts) {
         Vec8<T> x;
         x.load(p + (int64_t)s * a.Hkv * D);
 #pragma unroll
@@ -220,10 +237,10 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
     for (int j = 0; j < 8; ++j) part[tid * 8 + j] = acc[j];
     __syncthreads();
     const int e = tid;  // 32 chunks x 8 elements
-    if (cb * 8 + e < chunks * 8) {
+    if (e < 256 && cb * 8 + e < chunks * 8) {
       float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += part[i * 256 + e];
+      for (int i = 0; i < kSumParts; ++i) s += part[i * 256 + e];
       a.sums[(int64_t)ph * a.Hkv * D + cb * 8 + e] = s;
     }
     __syncthreads();
@@ -383,8 +400,13 @@ struct Step {
   }
 };
 
+// Waves per SIMD that the registers are budgeted for; two or more also keep the
+// products out of the accumulation registers.
+template <typename T, int DP>
+constexpr int kDecOcc = DP * (int)sizeof(T) > 256 ? 1 : (DP * (int)sizeof(T) > 128 ? 2 : 3);
+
 template <typename T, int DP, bool FULL>
-__global__ __launch_bounds__(64 * kDecWaves) void decode_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(64 * kDecWaves, (kDecOcc<T, DP>)) void decode_kernel(DecodeArgs a) {
   using St = Step<T, DP, FULL>;
   constexpr bool k16 = sizeof(T) == 2;
   constexpr int NK = St::NK, VPL = St::VPL;
@@ -587,65 +609,74 @@ __global__ __launch_bounds__(64 * kDecWaves) void decode_kernel(DecodeArgs a) {
 }
 
 // Joins the splits of one (stream, head): o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.
-constexpr int kJoinThreads = 256;
+// 1024 / DT groups of DT threads take every group-th split; a thread's first
+// eight outputs are under way before the weights are known.
+constexpr int kJoinThreads = 1024;
 constexpr int kMaxSplit = 256;
 
-template <typename T>
+template <typename T, int DT>
 __global__ __launch_bounds__(kJoinThreads) void decode_join_kernel(DecodeArgs a) {
+  constexpr int NG = kJoinThreads / DT;
   __shared__ float s_f[kMaxSplit];
   __shared__ float s_red[kJoinThreads];
-  __shared__ float s_stat[3];
-  const int tid = threadIdx.x;
+  __shared__ float s_m[kMaxSplit / 64], s_l[kMaxSplit / 64];
+  __shared__ int s_any[kMaxSplit / 64];
+  const int tid = threadIdx.x, w = tid >> 6;
   const int64_t row = blockIdx.x;
   const float* ml = a.part_ml + row * a.nsplit * 2;
-  if (tid < 64) {
-    float M = -INFINITY;
-    int any = 0;
-    for (int s = tid; s < a.nsplit; s += 64) {
-      M = fmaxf(M, ml[2 * s]);
-      any |= ml[2 * s + 1] != -1.0f;
-    }
+  const int D = a.D, d = tid % DT, gr = tid / DT;
+  const float* po = a.part_o + row * a.nsplit * D + (d < D ? d : 0);
+  float x[8];
 #pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
-    any = __ballot(any) != 0;
-    const float mu = M == -INFINITY ? 0.0f : M;
-    float lt = 0.0f;
-    for (int s = tid; s < a.nsplit; s += 64) {
-      const float ls = ml[2 * s + 1];
-      const float f = ls == -1.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * s] - mu);
-      s_f[s] = f;
-      lt += ls == -1.0f ? 0.0f : f * ls;
+  for (int i = 0; i < 8; ++i) x[i] = gr + i * NG < a.nsplit ? po[(int64_t)(gr + i * NG) * D] : 0.0f;
+  // statistics: thread s < 256 has split s
+  float M = -INFINITY, ls = -1.0f;
+  if (tid < kMaxSplit) {
+    if (tid < a.nsplit) {
+      M = ml[2 * tid];
+      ls = ml[2 * tid + 1];
     }
+    float mw = M;
 #pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) lt += __shfl_xor(lt, k, 64);
-    if (tid == 0) {
-      s_stat[0] = M;
-      s_stat[1] = lt;
-      s_stat[2] = any ? 1.0f : 0.0f;
+    for (int k = 32; k >= 1; k >>= 1) mw = fmaxf(mw, __shfl_xor(mw, k, 64));
+    const bool any = __ballot(ls != -1.0f) != 0;  // -1: the split has no key
+    if ((tid & 63) == 0) {
+      s_m[w] = mw;
+      s_any[w] = any;
     }
   }
   __syncthreads();
-  // 256 / dt groups of dt threads take every group-th split
-  const int D = a.D, dt = D <= 32 ? 32 : (D <= 64 ? 64 : 128), ng = kJoinThreads / dt;
-  const int d = tid % dt, gr = tid / dt;
+  const float Mt = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float mu = Mt == -INFINITY ? 0.0f : Mt;
+  const bool any = (s_any[0] | s_any[1] | s_any[2] | s_any[3]) != 0;
+  if (tid < kMaxSplit) {
+    const float f = ls == -1.0f ? 0.0f : __builtin_amdgcn_exp2f(M - mu);
+    s_f[tid] = ls == -1.0f ? -1.0f : f;
+    float l = ls == -1.0f ? 0.0f : f * ls;
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) l += __shfl_xor(l, k, 64);
+    if ((tid & 63) == 0) s_l[w] = l;
+  }
+  __syncthreads();
+  const float lt = s_l[0] + s_l[1] + s_l[2] + s_l[3];
   float o = 0.0f;
-  if (d < D) {
-    const float* po = a.part_o + row * a.nsplit * D + d;
-#pragma unroll 8
-    for (int s = gr; s < a.nsplit; s += ng) {
-      const float f = s_f[s];
-      // a split without keys has no output
-      o += f == 0.0f && ml[2 * s + 1] == -1.0f ? 0.0f : f * po[(int64_t)s * D];
-    }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int s = gr + i * NG;
+    const float f = s < a.nsplit ? s_f[s] : -1.0f;
+    if (f >= 0.0f || f != f) o += f * x[i];  // a split without keys has no output
+  }
+  for (int s = gr + 8 * NG; s < a.nsplit; s += NG) {
+    const float f = s_f[s];
+    if (f >= 0.0f || f != f) o += f * po[(int64_t)s * D];
   }
   s_red[tid] = o;
   __syncthreads();
   if (gr == 0 && d < D) {
-    for (int i = 1; i < ng; ++i) o += s_red[i * dt + d];
-    const bool any = s_stat[2] != 0.0f;
-    static_cast<T*>(a.out)[row * D + d] = static_cast<T>(any ? o / s_stat[1] : 0.0f);
-    if (a.lse && d == 0)
-      a.lse[row] = any ? s_stat[0] + (__log2f(s_stat[1]) - WeightPlanes<T>::kBias) : -INFINITY;
+#pragma unroll
+    for (int i = 1; i < NG; ++i) o += s_red[i * DT + d];
+    static_cast<T*>(a.out)[row * D + d] = static_cast<T>(any ? o / lt : 0.0f);
+    if (a.lse && d == 0) a.lse[row] = any ? Mt + (__log2f(lt) - WeightPlanes<T>::kBias) : -INFINITY;
   }
 }
 

@@ -96,11 +96,25 @@ class PagedCache:
             raise RuntimeError("head_dim must be a multiple of 8 from 8 to 128, with at least one head")
         if sums is not None:
             _tensors("key_sums", sums, torch.float32, 3, (P, Hkv, D), key.device)
-        self.key, self.value, self.key_sums = key, value, sums
+        self._key, self._value, self._sums = key, value, sums
+        self._descs = {}  # descriptors of calls on this cache, by the calls' sizes
+
+    # the tensors stay the checked ones
+    @property
+    def key(self) -> torch.Tensor:
+        return self._key
+
+    @property
+    def value(self) -> torch.Tensor:
+        return self._value
+
+    @property
+    def key_sums(self) -> Optional[torch.Tensor]:
+        return self._sums
 
     @property
     def page_size(self) -> int:
-        return int(self.key.shape[1])
+        return int(self._key.shape[1])
 
 
 class Rotation:
@@ -142,39 +156,80 @@ def _tensors(name, t, dtype, dim, shape=None, device=None) -> None:
         raise RuntimeError(f"{name} is on another device than the cache")
 
 
+def _valid(dtype, dev: int, *ts) -> bool:
+    """Whether the tensors are contiguous, of one dtype, on device `dev`: with the
+    shapes, the common valid call; any failure takes the ordered checks."""
+    try:
+        for t in ts:
+            if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+                return False
+        return dev >= 0
+    except AttributeError:
+        return False
+
+
 def _int32(name, t, shape, cache) -> None:
-    _tensors(name, t, torch.int32, len(shape), shape, cache.key.device)
+    _tensors(name, t, torch.int32, len(shape), shape, cache._key.device)
 
 
 def _table(page_table, B, cache) -> None:
-    _tensors("page_table", page_table, torch.int32, 2, None, cache.key.device)
+    _tensors("page_table", page_table, torch.int32, 2, None, cache._key.device)
     if page_table.shape[0] != B:
         raise RuntimeError(f"page_table must have a row per stream ({B}), got {page_table.shape[0]}")
 
 
-def _desc(cache, B, H, table, **kw) -> _Desc:
-    P, ps, Hkv, D = cache.key.shape
-    if H < 1 or H % Hkv:
-        raise RuntimeError(f"query heads ({H}) must be a multiple of the cache's heads ({Hkv})")
-    d = _Desc(batch=B, num_heads=H, num_kv_heads=Hkv, head_dim=D, num_pages=P, page_size=ps,
-              table_width=table.shape[1], dtype=_ma.DTYPES[cache.key.dtype], left=-1)
-    for k, v in kw.items():
-        setattr(d, k, v)
+def _desc(cache, key, B, H, width, workspace=None, **kw):
+    """(descriptor, workspace bytes) of a call, kept with the cache per `key` (the
+    call's sizes); a call with kernel events gets its own."""
+    hit = cache._descs.get(key)
+    if hit is None:
+        P, ps, Hkv, D = cache._key.shape
+        if H < 1 or H % Hkv:
+            raise RuntimeError(f"query heads ({H}) must be a multiple of the cache's heads ({Hkv})")
+        d = _Desc(batch=B, num_heads=H, num_kv_heads=Hkv, head_dim=D, num_pages=P, page_size=ps, table_width=width,
+                  dtype=_ma.DTYPES[cache._key.dtype], left=-1)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        if len(cache._descs) > 256:
+            cache._descs.clear()
+        hit = cache._descs[key] = (d, int(workspace(ctypes.byref(d))) if workspace else 0)
     if _ext._events is not None:
+        d = _Desc.from_buffer_copy(hit[0])
         d.start_event, d.stop_event = (e or None for e in _ext._events)
-    return d
+        return d, hit[1]
+    return hit
+
+
+def _ptr(t) -> Optional[int]:
+    return t.data_ptr() or None if t is not None else None
 
 
 def _call(fn, dev: int, *args) -> None:
-    ptrs = [a.data_ptr() or None if isinstance(a, torch.Tensor) else a for a in args]
-    rc = _ext._on_device(dev, lambda stream: fn(*ptrs, stream or None))
-    if rc != 0:
+    if _ext._on_device(dev, lambda stream: fn(*args, stream or None)) != 0:
         raise RuntimeError(_ma.last_error())
 
 
 def _check_cache(cache) -> None:
     if not isinstance(cache, PagedCache):
         raise RuntimeError("cache must be a PagedCache")
+
+
+def _check_append(cache, key, value, page_table, start, counts, query) -> None:
+    dev = cache._key.device
+    _tensors("key", key, cache._key.dtype, 4, None, dev)
+    B, N = key.shape[:2]
+    Hkv, D = cache._key.shape[2:]
+    if tuple(key.shape[2:]) != (Hkv, D):
+        raise RuntimeError(f"key must be [B, N, {Hkv}, {D}] as the cache, got {tuple(key.shape)}")
+    _tensors("value", value, cache._key.dtype, 4, key.shape, dev)
+    _table(page_table, B, cache)
+    _int32("start", start, (B,), cache)
+    if counts is not None:
+        _int32("counts", counts, (B,), cache)
+    if query is not None:
+        _tensors("query", query, cache._key.dtype, 4, None, dev)
+        if tuple(query.shape[:2]) != (B, N) or query.shape[3] != D:
+            raise RuntimeError(f"query must be [{B}, {N}, H, {D}], got {tuple(query.shape)}")
 
 
 def paged_append(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor,
@@ -191,48 +246,49 @@ def paged_append(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, page
     a page may read it, not append to it in one call.
     """
     _check_cache(cache)
-    dev = cache.key.device
-    _tensors("key", key, cache.key.dtype, 4, None, dev)
-    B, N = key.shape[:2]
-    Hkv, D = cache.key.shape[2:]
-    if tuple(key.shape[2:]) != (Hkv, D):
-        raise RuntimeError(f"key must be [B, N, {Hkv}, {D}] as the cache, got {tuple(key.shape)}")
-    _tensors("value", value, cache.key.dtype, 4, key.shape, dev)
-    _table(page_table, B, cache)
-    _int32("start", start, (B,), cache)
-    if counts is not None:
-        _int32("counts", counts, (B,), cache)
-    H, out = Hkv, None
-    if query is not None:
-        _tensors("query", query, cache.key.dtype, 4, None, dev)
-        if tuple(query.shape[:2]) != (B, N) or query.shape[3] != D:
-            raise RuntimeError(f"query must be [{B}, {N}, H, {D}], got {tuple(query.shape)}")
-        H = query.shape[2]
-        out = torch.empty_like(query)
+    ck = cache._key
+    dev = ck.get_device()
+    q = key if query is None else query
+    n = start if counts is None else counts
+    if not (_valid(ck.dtype, dev, key, value, q) and _valid(torch.int32, dev, page_table, start, n)
+            and key.dim() == 4 and q.dim() == 4 and page_table.dim() == 2 and start.dim() == 1
+            and value.shape == key.shape and n.shape == start.shape
+            and key.shape[2:] == ck.shape[2:] and (q is key or (q.shape[:2] == key.shape[:2] and q.shape[3] == ck.shape[3]))
+            and page_table.shape[0] == start.shape[0] == key.shape[0]):
+        _check_append(cache, key, value, page_table, start, counts, query)
+    B, N, Hkv, D = key.shape
+    H = q.shape[2]
+    out = torch.empty_like(query) if query is not None else None
     freq, kw = None, {}
     if rotation is not None:
         if not isinstance(rotation, Rotation):
             raise RuntimeError("rotation must be a Rotation")
         if rotation.dim > D:
             raise RuntimeError(f"rotation dim ({rotation.dim}) exceeds head_dim ({D})")
-        if rotation.inv_freq.device != dev:
+        if rotation.inv_freq.device != ck.device:
             raise RuntimeError("rotation is on another device than the cache")
         freq, kw = rotation.inv_freq, dict(rotary_dim=rotation.dim, interleaved=int(rotation.interleaved))
-    d = _desc(cache, B, H, page_table, num_tokens=N, **kw)
-    _call(_lib.ma_paged_append, dev.index, ctypes.byref(d), key, value, query, out, cache.key, cache.value,
-          cache.key_sums, page_table, start, counts, freq)
+    width = page_table.shape[1]
+    d, _ = _desc(cache, ("append", B, N, H, width, *kw.values()), B, H, width, num_tokens=N, **kw)
+    _call(_lib.ma_paged_append, dev, ctypes.byref(d), key.data_ptr(), value.data_ptr(), _ptr(query),
+          _ptr(out), cache._key.data_ptr(), cache._value.data_ptr(), _ptr(cache._sums), page_table.data_ptr(),
+          start.data_ptr(), _ptr(counts), _ptr(freq))
     return out
 
 
 def _query(query, cache, page_table, lengths):
     _check_cache(cache)
-    _tensors("query", query, cache.key.dtype, 3, None, cache.key.device)
-    B, H, D = query.shape
-    if D != cache.key.shape[3]:
-        raise RuntimeError(f"query head_dim ({D}) must be the cache's ({cache.key.shape[3]})")
-    _table(page_table, B, cache)
-    _int32("lengths", lengths, (B,), cache)
-    return B, H, D
+    ck = cache._key
+    dev = ck.get_device()
+    if not (_valid(ck.dtype, dev, query) and _valid(torch.int32, dev, page_table, lengths) and query.dim() == 3
+            and page_table.dim() == 2 and lengths.dim() == 1 and query.shape[2] == ck.shape[3]
+            and page_table.shape[0] == lengths.shape[0] == query.shape[0]):
+        _tensors("query", query, ck.dtype, 3, None, ck.device)
+        if query.shape[2] != ck.shape[3]:
+            raise RuntimeError(f"query head_dim ({query.shape[2]}) must be the cache's ({ck.shape[3]})")
+        _table(page_table, query.shape[0], cache)
+        _int32("lengths", lengths, (query.shape[0],), cache)
+    return query.shape
 
 
 def paged_decode(query: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -250,29 +306,32 @@ def paged_decode(query: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     1/sqrt(head_dim)).
     """
     B, H, D = _query(query, cache, page_table, lengths)
-    kw = {**_ext._scale_kw(scale)}
+    S, num_global = 0, int(num_global)
     if left is not None:
-        if int(left) < 0:
+        left = int(left)
+        if left < 0:
             raise RuntimeError("left must be >= 0")
-        kw["left"] = min(int(left), 1 << 62)
-    if int(num_global) < 0 or (int(num_global) > 0 and left is None):
+    if num_global < 0 or (num_global > 0 and left is None):
         raise RuntimeError("num_global must be >= 0 and goes with left")
-    kw["num_global"] = min(int(num_global), 1 << 62)
     if pages is not None:
         if left is not None:
             raise RuntimeError("pages and left exclude each other")
-        _tensors("pages", pages, torch.int32, 3, None, cache.key.device)
-        if tuple(pages.shape[:2]) != (B, cache.key.shape[2]) or not 1 <= pages.shape[2] <= 64:
-            raise RuntimeError(f"pages must be [{B}, {cache.key.shape[2]}, S] with 1 <= S <= 64, "
+        _tensors("pages", pages, torch.int32, 3, None, cache._key.device)
+        S = pages.shape[2]
+        if pages.shape[:2] != (B, cache._key.shape[2]) or not 1 <= S <= 64:
+            raise RuntimeError(f"pages must be [{B}, {cache._key.shape[2]}, S] with 1 <= S <= 64, "
                                f"got {tuple(pages.shape)}")
-        kw["num_selected"] = pages.shape[2]
-    d = _desc(cache, B, H, page_table, **kw)
+    kw = _ext._scale_kw(scale)
+    width = page_table.shape[1]
+    d, nbytes = _desc(cache, ("decode", B, H, width, left, num_global, S, kw.get("scale")), B, H, width,
+                      _lib.ma_paged_decode_workspace_size, left=-1 if left is None else min(left, 1 << 62),
+                      num_global=min(num_global, 1 << 62), num_selected=S, **kw)
     out = torch.empty_like(query)
     lse = torch.empty((B, H), dtype=torch.float32, device=query.device) if return_lse else None
-    nbytes = int(_lib.ma_paged_decode_workspace_size(ctypes.byref(d)))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
-    _call(_lib.ma_paged_decode, query.get_device(), ctypes.byref(d), query, cache.key, cache.value, page_table,
-          lengths, pages, out, lse, ws, nbytes)
+    _call(_lib.ma_paged_decode, query.get_device(), ctypes.byref(d), query.data_ptr(), cache._key.data_ptr(),
+          cache._value.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _ptr(pages), out.data_ptr(), _ptr(lse),
+          _ptr(ws), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -287,14 +346,17 @@ def paged_select(query: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     page and NaN scores rank last.  At most 16384 pages a stream.
     """
     B, H, D = _query(query, cache, page_table, lengths)
-    if cache.key_sums is None:
+    if cache._sums is None:
         raise RuntimeError("paged_select needs a cache with key_sums")
     S, first, local = int(num_selected), int(first_pages), int(local_pages)
     if not 1 <= S <= 64:
         raise RuntimeError("num_selected must be in [1, 64]")
     if first < 0 or local < 1 or first + local > S:
         raise RuntimeError("first_pages >= 0 and local_pages >= 1 must fit in num_selected")
-    d = _desc(cache, B, H, page_table, num_selected=S, first_pages=first, local_pages=local)
-    out = torch.empty((B, cache.key.shape[2], S), dtype=torch.int32, device=query.device)
-    _call(_lib.ma_paged_select, query.get_device(), ctypes.byref(d), query, cache.key_sums, page_table, lengths, out)
+    width = page_table.shape[1]
+    d, _ = _desc(cache, ("select", B, H, width, S, first, local), B, H, width, num_selected=S, first_pages=first,
+                 local_pages=local)
+    out = torch.empty((B, cache._key.shape[2], S), dtype=torch.int32, device=query.device)
+    _call(_lib.ma_paged_select, query.get_device(), ctypes.byref(d), query.data_ptr(), cache._sums.data_ptr(),
+          page_table.data_ptr(), lengths.data_ptr(), out.data_ptr())
     return out

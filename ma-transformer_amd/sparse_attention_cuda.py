@@ -611,6 +611,18 @@ for _name, _nptr in (("select_blocks", 3), ("selected_forward", 6), ("selected_b
 
 def _check_selected(q: torch.Tensor, *kv: torch.Tensor) -> None:
     """q [B, S, H, D], the others [B, S, Hkv, D] with H a multiple of Hkv."""
+    # one pass for the common valid call; any failure takes the ordered checks below
+    try:
+        shape, dt, dev = kv[0].shape, q.dtype, q.get_device()
+        ok = (dt in _ma.DTYPES and dev >= 0 and len(shape) == 4 and q.is_contiguous() and q.dim() == 4
+              and shape[2] >= 1 and q.shape[2] >= 1 and q.shape[2] % shape[2] == 0
+              and (q.shape[0], q.shape[1], q.shape[3]) == (shape[0], shape[1], shape[3]))
+        for t in kv:
+            ok = ok and t.dtype is dt and t.shape == shape and t.is_contiguous() and t.get_device() == dev
+        if ok:
+            return
+    except (AttributeError, TypeError, IndexError):
+        pass
     for t in (q, *kv):
         if not isinstance(t, torch.Tensor):
             raise RuntimeError("Inputs must be tensors")
@@ -635,21 +647,33 @@ def _check_selected(q: torch.Tensor, *kv: torch.Tensor) -> None:
         raise RuntimeError(f"query heads ({H}) must be a multiple of key/value heads ({Hkv})")
 
 
-def _select_desc(q, k, block_size, num_selected, causal, **kw):
-    B, N, H, D = q.shape
-    d = _SelectDesc(batch=B, seq_len=N, num_heads=H, num_kv_heads=k.shape[2], head_dim=D, block_size=int(block_size),
-                    num_selected=int(num_selected), dtype=_ma.DTYPES[q.dtype], causal=int(bool(causal)), **kw)
+_select_cache: dict = {}
+
+
+def _select_desc(name, q, k, block_size, num_selected, causal, **kw):
+    """(descriptor, workspace bytes), kept per call signature."""
+    sig = (name, q.shape, k.shape[2], q.dtype, block_size, num_selected, causal, *kw.values())
+    hit = _select_cache.get(sig)
+    if hit is None:
+        B, N, H, D = q.shape
+        d = _SelectDesc(batch=B, seq_len=N, num_heads=H, num_kv_heads=k.shape[2], head_dim=D, block_size=block_size,
+                        num_selected=num_selected, dtype=_ma.DTYPES[q.dtype], causal=causal, **kw)
+        if len(_select_cache) > 256:
+            _select_cache.clear()
+        hit = _select_cache[sig] = (d, int(getattr(_ma.LIB, f"ma_{name}_workspace_size")(ctypes.byref(d))))
     if _events is not None:
+        d = _SelectDesc.from_buffer_copy(hit[0])
         d.start_event, d.stop_event = (e or None for e in _events)
-    return d
+        return d, hit[1]
+    return hit
 
 
-def _call_selected(name: str, d: _SelectDesc, dev: int, device, *ptrs) -> None:
-    nbytes = int(getattr(_ma.LIB, f"ma_{name}_workspace_size")(ctypes.byref(d)))
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
-    args = [p.data_ptr() or None if isinstance(p, torch.Tensor) else p for p in ptrs]
+def _call_selected(name: str, desc, q, *ptrs) -> None:
+    d, nbytes = desc
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+    args = [p.data_ptr() or None if p is not None else None for p in ptrs]
     fn = getattr(_ma.LIB, "ma_" + name)
-    if _on_device(dev, lambda stream: fn(ctypes.byref(d), *args, ws.data_ptr(), nbytes, stream or None)) != 0:
+    if _on_device(q.get_device(), lambda stream: fn(ctypes.byref(d), *args, ws.data_ptr(), nbytes, stream or None)):
         raise RuntimeError(_ma.last_error())
 
 
@@ -672,10 +696,11 @@ def select_blocks(query: torch.Tensor, key: torch.Tensor, num_selected: int, blo
         raise RuntimeError("num_selected must be in [1, 64]")
     if first < 0 or local < 1 or first + local > S:
         raise RuntimeError("first_blocks >= 0 and local_blocks >= 1 must fit in num_selected")
-    d = _select_desc(query, key, block_size, S, causal, first_blocks=first, local_blocks=local)
+    d = _select_desc("select_blocks", query, key, int(block_size), S, int(bool(causal)), first_blocks=first,
+                     local_blocks=local)
     B, N, Hkv, _ = key.shape
     out = torch.empty((B, N, Hkv, S), dtype=torch.int32, device=query.device)
-    _call_selected("select_blocks", d, query.get_device(), query.device, query, key, out)
+    _call_selected("select_blocks", d, query, query, key, out)
     return out
 
 
@@ -701,10 +726,11 @@ def selected_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     one)."""
     _check_selected(query, key, value)
     _check_blocks(blocks, key)
-    d = _select_desc(query, key, block_size, blocks.shape[3], causal, **_scale_kw(scale))
+    d = _select_desc("selected_forward", query, key, int(block_size), blocks.shape[3], int(bool(causal)),
+                     **_scale_kw(scale))
     out = torch.empty_like(query)
     lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device) if return_lse else None
-    _call_selected("selected_forward", d, query.get_device(), query.device, query, key, value, blocks, out, lse)
+    _call_selected("selected_forward", d, query, query, key, value, blocks, out, lse)
     return (out, lse) if return_lse else out
 
 
@@ -721,8 +747,8 @@ def selected_backward(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
         out, lse = selected_forward(query, key, value, blocks, block_size, causal, True, scale)
     _check(query, out)
     _check_lse(lse, query)
-    d = _select_desc(query, key, block_size, blocks.shape[3], causal, **_scale_kw(scale))
+    d = _select_desc("selected_backward", query, key, int(block_size), blocks.shape[3], int(bool(causal)),
+                     **_scale_kw(scale))
     dq, dk, dv = (torch.empty_like(t) for t in (query, key, value))
-    _call_selected("selected_backward", d, query.get_device(), query.device, query, key, value, blocks, out, lse,
-                   grad_out, dq, dk, dv)
+    _call_selected("selected_backward", d, query, query, key, value, blocks, out, lse, grad_out, dq, dk, dv)
     return [dq, dk, dv]
