@@ -85,7 +85,7 @@ struct RowLds {
 inline size_t row_lds_bytes(int S) { return kRowWaves * (sizeof(RowLds) + (size_t)16 * S * 8); }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args a) {
+__global__ __launch_bounds__(64 * kRowWaves, 2) void rows_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   constexpr int SD = DP / 4;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -140,16 +140,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args a) {
         }
       }
     }
-    // carried blocks: slot 4 r + g of the query's list
-    uint32_t ck[16];
-    int32_t ci[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const bool in = 4 * r + g < have;
-      ck[r] = in ? lk[c * S + 4 * r + g] : 0u;
-      ci[r] = in ? li[c * S + 4 * r + g] : 0;
-    }
+    // carried blocks, in the query's list: slot 4 r + g
     const bool carried = t0 > 0;
+    auto ckey = [&](int r) { return 4 * r + g < have ? lk[c * S + 4 * r + g] : 0u; };
+    auto cblk = [&](int r) { return 4 * r + g < have ? li[c * S + 4 * r + g] : 0; };
+    const int cr = (S + 3) >> 2;
     auto sum4 = [&](int x) {
       x += __shfl_xor(x, 16, 64);
       return x + __shfl_xor(x, 32, 64);
@@ -161,8 +156,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) n += key[u][r] >= th;
       if (carried)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) n += ck[r] >= th;
+        for (int r = 0; r < cr; ++r) n += ckey(r) >= th;
       return sum4(n);
     };
     // the largest threshold that at least S keys reach
@@ -176,8 +170,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) see(key[u][r]);
     if (carried)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) see(ck[r]);
+      for (int r = 0; r < cr; ++r) see(ckey(r));
     for (int k = 16; k < 64; k <<= 1) {
       const uint32_t x = __shfl_xor(mx, k, 64), y = __shfl_xor(mn, k, 64);
       mx = x > mx ? x : mx;
@@ -230,8 +223,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args a) {
         m += __popcll(bal);
       };
       if (carried)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) collect(ck[r], ci[r]);
+        for (int r = 0; r < cr; ++r) collect(ckey(r), cblk(r));
 #pragma unroll
       for (int u = 0; u < kChunkTiles; ++u)
 #pragma unroll
@@ -275,8 +267,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args a) {
         m += __popcll(bal);
       };
       if (carried)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) drop(ck[r]);
+        for (int r = 0; r < cr; ++r) {
+          uint32_t k = ckey(r);
+          drop(k);
+          if (4 * r + g < have) lk[c * S + 4 * r + g] = k;
+        }
 #pragma unroll
       for (int u = 0; u < kChunkTiles; ++u)
 #pragma unroll
@@ -298,8 +293,13 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args a) {
     };
     wave_fence();
     if (carried)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) keep(ck[r], ci[r]);
+      for (int r = 0; r < cr; ++r) {  // in place: nothing moves up
+        const uint32_t k = ckey(r);
+        const int32_t blk = cblk(r);
+        wave_fence();
+        keep(k, blk);
+        wave_fence();
+      }
 #pragma unroll
     for (int u = 0; u < kChunkTiles; ++u)
 #pragma unroll
