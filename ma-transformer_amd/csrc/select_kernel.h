@@ -45,14 +45,13 @@ __global__ __launch_bounds__(kMeanThreads) void mean_kernel(Args a, int parts) {
 
 // Ordered 32-bit key of a score rounded to float32 (the rounding keeps the
 // order, weakly); 0: may not be listed, ~0: always listed.
-__device__ __forceinline__ uint32_t key32(double x) {
-  x = x != x ? -__builtin_inf() : x + 0.0;
-  const uint32_t u = __float_as_uint((float)x);
-  return u >> 31 ? ~u : u | 0x80000000u;
-}
 __device__ __forceinline__ uint32_t key32f(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return u >> 31 ? ~u : u | 0x80000000u;
+  const int u = __float_as_int(x);
+  return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint32_t key32(double x) {
+  const float f = (float)x;
+  return key32f(f != f ? -INFINITY : f + 0.0f);
 }
 __device__ __forceinline__ float value32(uint32_t k) {
   return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k);
@@ -115,6 +114,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void rows_kernel(Args a) {
   const int64_t ilast = i0 + 15 < a.N ? i0 + 15 : a.N - 1;
   const int nt = a.causal ? (int)(ilast / a.BS) / 16 + 1 : a.nbp / 16;
   int have = 0;  // listed so far (carried)
+  const int own_first = (int)(i0 / a.BS);  // the first query's block: no query's is lower
   for (int t0 = 0; t0 < nt; t0 += kChunkTiles) {
     uint32_t key[kChunkTiles][4];
 #pragma unroll
@@ -132,11 +132,16 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void rows_kernel(Args a) {
           acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x.y, qs[s + 1], acc, 0, 0, 0);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int blk = 16 * (t0 + u) + 4 * r + g;  // float64 results: row 4 r + g
-          const bool cand = blk < a.nb && (!a.causal || blk <= own);
-          const bool forced = blk < a.first || (blk <= own && blk > own - a.local);
-          key[u][r] = cand ? (forced ? ~0u : key32(acc[r])) : 0u;
+        for (int r = 0; r < 4; ++r) key[u][r] = key32(acc[r]);
+        const int b0 = 16 * (t0 + u);
+        if (b0 < a.first || b0 + 15 > own_first - a.local) {  // not every block is an ordinary candidate
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int blk = b0 + 4 * r + g;  // float64 results: row 4 r + g
+            const bool cand = blk < a.nb && (!a.causal || blk <= own);
+            const bool forced = blk < a.first || (blk <= own && blk > own - a.local);
+            key[u][r] = cand ? (forced ? ~0u : key[u][r]) : 0u;
+          }
         }
       }
     }
@@ -152,9 +157,12 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void rows_kernel(Args a) {
     auto at_least = [&](uint32_t th) {
       int n = 0;
 #pragma unroll
-      for (int u = 0; u < kChunkTiles; ++u)
+      for (int q = 0; q < kChunkTiles; q += 4)
+        if (t0 + q < nt)  // four tiles at a time, as far as there are any
 #pragma unroll
-        for (int r = 0; r < 4; ++r) n += key[u][r] >= th;
+          for (int u = q; u < q + 4; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) n += key[u][r] >= th;
       if (carried)
         for (int r = 0; r < cr; ++r) n += ckey(r) >= th;
       return sum4(n);
@@ -166,9 +174,12 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void rows_kernel(Args a) {
       mn = k != 0 && k < mn ? k : mn;
     };
 #pragma unroll
-    for (int u = 0; u < kChunkTiles; ++u)
+    for (int q = 0; q < kChunkTiles; q += 4)
+      if (t0 + q < nt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) see(key[u][r]);
+        for (int u = q; u < q + 4; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) see(key[u][r]);
     if (carried)
       for (int r = 0; r < cr; ++r) see(ckey(r));
     for (int k = 16; k < 64; k <<= 1) {
@@ -187,9 +198,9 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void rows_kernel(Args a) {
     for (int step = 0; __ballot(!done); ++step) {
       uint32_t mid = lo + ((hi - lo) >> 1);
       const float fl = value32(lo), fh = value32(hi);
-      // halving the values converges faster than halving the keys on ordinary
-      // scores; every third step halves the keys, which always ends
-      if (step % 3 != 2 && fabsf(fl) < 1e30f && fabsf(fh) < 1e30f) mid = key32f(0.5f * (fl + fh) + 0.0f);
+      // halving the values converges in about 12 steps on ordinary scores; from
+      // the 16th on the keys are halved, which ends in 32
+      if (step < 16 && fabsf(fl) < 1e30f && fabsf(fh) < 1e30f) mid = key32f(0.5f * (fl + fh) + 0.0f);
       mid = mid <= lo ? lo + 1 : (mid >= hi ? hi - 1 : mid);
       if (!done && hi - lo <= 1) {
         thr = lo;
@@ -301,9 +312,12 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void rows_kernel(Args a) {
         wave_fence();
       }
 #pragma unroll
-    for (int u = 0; u < kChunkTiles; ++u)
+    for (int q = 0; q < kChunkTiles; q += 4)
+      if (t0 + q < nt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) keep(key[u][r], 16 * (t0 + u) + 4 * r + g);
+        for (int u = q; u < q + 4; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) keep(key[u][r], 16 * (t0 + u) + 4 * r + g);
     have = put < S ? put : S;
     wave_fence();
   }
