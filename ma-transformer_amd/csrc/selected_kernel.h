@@ -212,7 +212,12 @@ __global__ __launch_bounds__(kListThreads) void fill_kernel(Args a) {
 // O^T = V^T P^T, so statistics and weights never leave their lane.
 //
 // Bound by the partial rows (one float32 row of head_dim per pair and head,
-// written here and read by the join).
+// written here and read by the join): without its stores the kernel takes 107
+// us where it takes 135 to 150 (8 heads of 16384 rows, 16 of 64 keys, bf16: 537
+// MB of partial rows, 4.0 TB/s).  They go through LDS so that a store writes
+// whole rows, and past the caches (non-temporal): half rows stored from the
+// result layout took 230 us, whole rows 205, and the join reads them in 125
+// instead of 145.
 
 constexpr int kFwdWaves = 4;
 
@@ -347,8 +352,7 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
   const float sl2 = a.scale_log2;
 
   // a row past the end repeats the last one and stores the same values to the
-  // same place: memory operations under a branch would make the wait for the
-  // next queries one for these stores too (230 -> 150 us)
+  // same place, so that no store stands under a branch
   auto entry_of = [&](int r) { return list[(a.G == 1 ? r : r / a.G)]; };
   auto head_of = [&](int r) { return a.G == 1 ? 0 : r % a.G; };
   auto clamp = [&](int r) { return r < rows ? r : rows - 1; };
@@ -363,7 +367,7 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
     for (int i = 0; i < NK; ++i) f[i] = FULL || 32 * i + 8 * g < D ? O::load(p + 32 * i + 8 * g) : O::zero();
   };
   load_q(qf, ent, gh);
-  auto tile = [&](int t0) {
+  for (int t0 = 16 * w; t0 < rows; t0 += STEP) {
     const int ghn = head_of(clamp(t0 + STEP + c));
     const int ent2 = entry_of(clamp(t0 + 2 * STEP + c));
     f32x4 s[NT];
@@ -470,13 +474,7 @@ __global__ __launch_bounds__(64 * kFwdWaves, (kFwdOcc<T, DP, NT>)) void forward_
     ent = entn;
     entn = ent2;
     gh = ghn;
-  };
-  // the first tile stands before the loop, which is then entered as it repeats:
-  // with the next queries under way and this tile's stores behind them.  Where
-  // the two ways in differ the compiler waits for the lesser count, and with it
-  // for stores.
-  tile(16 * w);
-  for (int t0 = 16 * w + STEP; t0 < rows; t0 += STEP) tile(t0);
+  }
 }
 
 // ---------------------------------------------------------------- joining a query's slots
@@ -646,7 +644,10 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
   constexpr int JD = (ND + NT - 1) / NT, KC = (NT + 1) / 2;
   static_assert(RT <= TH && RT % 32 == 0, "a thread per row of the tile");
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int x = (int)blockIdx.x;
+  // whole units per XCD, whose L2 then holds their Q and dO (8 units of 16384
+  // rows: training step 820 -> 790 us; 8 of 4095: 421 -> 424).  Other counts
+  // would give one XCD a unit's first blocks, which have the longest lists.
+  const int x = a.units % 8 == 0 ? xcd_row_order((int)blockIdx.x, (int)gridDim.x) : (int)blockIdx.x;
   const int ug = x / a.max_items, unit = a.unit0 + ug, slot_item = x % a.max_items;
   const int4 item = a.items[(int64_t)unit * a.max_items + slot_item];
   if (item.z < 0) return;
@@ -722,10 +723,9 @@ __global__ __launch_bounds__(64 * NT, (kBwdOcc<T, DP, NT>)) void backward_kernel
     const int rt = r0 + (tid & (RT - 1));
     est = pair_of(rt < rows ? rt : rows - 1);
   };
-  // no load and no store of the loop stands under a branch (rows past the end
-  // load the last row, and store their dQ to a row that nothing reads): the
-  // wait for the next tile's rows would otherwise be one for this tile's
-  // stores too
+  // no load and no store of the loop stands under a branch: rows past the end
+  // load the last row, and store their dQ to a row that nothing reads (training
+  // step of 2 x 8 heads on 4 of 4095 rows, head_dim 128: 517 -> 475 us)
   auto fetch = [&](int r0) {
     sown = 0;
 #pragma unroll
