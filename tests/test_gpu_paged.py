@@ -72,6 +72,8 @@ APPEND = [
     ("f16", 40, 16, True, 1, 4, 128, 130, [1], None, True),
     ("bf16", 128, 64, False, 1, 12, 16, 17, [3, 9], None, False),
     ("f32", 24, 16, False, 2, 2, 64, 129, [0, 1 << 20], [129, 3], True),
+    ("bf16", 64, 64, False, 2, 4, 1024, 1500, [1000, 0], [1500, 24], True),  # pages longer than a tile of tokens
+    ("f16", 128, 128, False, 40, 80, 16, 18, [5], None, True),               # a token of more units than threads
 ]
 
 
@@ -260,6 +262,7 @@ DECODE = [
     ("f32", 4, 2, 48, 32, [333, 40, 17], 16, 20),    # globals that end inside a tile
     ("bf16", 8, 8, 64, 64, [2000, 100], 127, 16),
     ("bf16", 2, 2, 64, 16, [90], 1 << 40, 1 << 40),  # a window longer than any stream
+    ("f16", 4, 2, 64, 1024, [1025, 1500, 1], None, 0),
 ]
 
 

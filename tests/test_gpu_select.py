@@ -495,3 +495,56 @@ def test_refusals(ext):
         assert bl.shape == (*shape[:2], 2, 3)
         assert ext.selected_forward(x, x, x, bl).shape == shape
         assert all(t.shape == shape for t in ext.selected_backward(x, x, x, x, bl))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_padded_batch(ext, dt):
+    """Sequences padded behind their ends: the rows before are those of the
+    unpadded sequence (causal: nothing behind a row reaches it), bit by bit with
+    zeros behind them.  With NaN the rows of the block that holds the end are
+    summed key by key, in another order: they are held to the 64-bit result."""
+    B, N, n, H, D, bs, S = 2, 500, 333, 2, 64, 32, 4
+    q, k, v, g = (rnd(i, B, N, H, D, dtype=T[dt]) for i in range(1, 5))
+    short = [x[:, :n].contiguous() for x in (q, k, v, g)]
+    bl = ext.select_blocks(short[0], short[1], S, bs)
+    o, lse = ext.selected_forward(*short[:3], bl, bs, True, True)
+    grads = ext.selected_backward(*short[:3], short[3], bl, bs, True, o, lse)
+    for fill in (0.0, math.nan):
+        x = [t.clone() for t in (q, k, v, g)]
+        for t in x:
+            t[:, n:] = fill
+        if fill == 0.0:  # rows whose every score ties
+            full = ext.select_blocks(x[0], x[1], S, bs)
+            assert torch.equal(full.cpu(), select64(x[0], x[1], S, bs, True, 0, 1))
+        pad = torch.full((B, N, H, S), -1, dtype=torch.int32, device=DEV)
+        pad[:, :n] = bl
+        po, pl = ext.selected_forward(x[0], x[1], x[2], pad, bs, True, True)
+        pg = ext.selected_backward(x[0], x[1], x[2], x[3], pad, bs, True, po, pl)
+        ref = attend64(*short, bl, bs, True)
+        for name, a, b in zip(("o", "dq", "dk", "dv"), (po, *pg), (o, *grads)):
+            assert not bool(a[:, n:].any()), name
+            close(name, a[:, :n], ref[name])
+            if fill == 0.0:
+                assert same(a[:, :n].contiguous(), b), name
+
+
+def test_two_streams_at_once(ext):
+    """Two training steps in flight on two streams do not meet."""
+    sets = [[rnd(10 * j + i, 1, 3000, 4, 64, dtype=torch.float16) for i in range(4)] for j in range(2)]
+
+    def step(q, k, v, g):
+        bl = ext.select_blocks(q, k, 8)
+        o, l = ext.selected_forward(q, k, v, bl, return_lse=True)
+        return [o, *ext.selected_backward(q, k, v, g, bl, out=o, lse=l)]
+
+    ref = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(step(*s))
+        torch.cuda.synchronize()
+        for a, b in zip(got, ref):
+            assert all(same(x, y) for x, y in zip(a, b))
