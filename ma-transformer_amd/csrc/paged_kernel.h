@@ -24,6 +24,9 @@ using namespace ma_dev;
 // keys [0, end) back (cache-hot) and adds them in slot order classes.  The sum
 // depends on the page's contents alone, not on the calls that filled it: a
 // stream that is set back and appended to again needs no correction.
+//
+// Bound by bytes on a prompt: 4 x 8191 tokens (three quarters stored), 8 heads of
+// 64, f16 take 33 us, 169 MB at 5.0 TB/s; a single token's launch 6 us.
 
 struct AppendArgs {
   const void* k;
@@ -261,6 +264,8 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
 // Bound by the cache's bytes: one step's loads are in flight while the last is
 // computed, and the token range is split over enough workgroups to fill the
 // card; their (maximum, sum, output) partials are joined by a second kernel.
+// One stream of 65536 tokens, 8 heads of 64, f16: 26 us (5.2 TB/s) and 4.2 for
+// the join; 32 streams of up to 8192, 2 heads of 128, bf16: 36 us (5.4 TB/s).
 
 struct DecodeArgs {
   const void* q;
@@ -684,8 +689,8 @@ __global__ __launch_bounds__(kJoinThreads) void decode_join_kernel(DecodeArgs a)
 //
 // One workgroup per (stream, key/value head): eight lanes a page, the scores'
 // ordered 64-bit keys in LDS, then the num_selected largest by radix selection
-// (top_select.h).  Bound by the page sums' bytes; the selection's few passes
-// over LDS are latency.
+// (top_select.h).  Latency: 6 MB of page sums (32 streams of 256 pages, 4 heads)
+// would take 1.3 us, the kernel 11, most of it the selection's passes over LDS.
 
 struct SelectArgs {
   const void* q;

@@ -69,6 +69,9 @@ __device__ __forceinline__ void wave_fence() {
 // queries at once.  Blocks that tie in float32 at the border are compared in
 // float64 (a few queries in 10^5 on real scores; every one of a zero query).
 // Sequences of more blocks go chunk by chunk with the S best carried over.
+// 16384 queries of 8 heads of 64, 16 of 256 blocks of 64, bf16: 175 us, bound by
+// vector instructions (12 bisection steps over up to 64 keys a lane); the
+// products' floor at the card's float64 rate is 33.
 constexpr int kRowWaves = 4;
 constexpr int kChunkTiles = 16;
 constexpr int kTies = 64 + 16 * kChunkTiles;
