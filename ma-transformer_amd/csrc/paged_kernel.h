@@ -313,18 +313,24 @@ __device__ __forceinline__ Tile make_tile(const DecodeArgs& a, int64_t b, int64_
 struct KeySet {
   int64_t len, ws, ng, wbase;
   int32_t ntg, total, tpp;
-  const int32_t* list;
+  int32_t ent;  // listed pages: lane l has entry l, -1 where it is skipped
+  bool listed;
 
-  __device__ __forceinline__ void init(const DecodeArgs& a, int64_t b, int hk) {
+  __device__ __forceinline__ void init(const DecodeArgs& a, int64_t b, int hk, int lane) {
+    listed = a.pages != nullptr;
+    ent = -1;
+    if (listed && lane < a.S) ent = a.pages[(b * a.Hkv + hk) * a.S + lane];
     len = a.lengths[b];
     const int64_t cap = (int64_t)a.width * a.page;
     len = len < 0 ? 0 : (len > cap ? cap : len);
     tpp = a.page >> 4;
-    list = nullptr;
     ws = 0;
     ng = 0;
-    if (a.pages) {
-      list = a.pages + (b * a.Hkv + hk) * a.S;
+    if (listed) {
+      for (int j = 0; j + 1 < a.S; ++j) {  // repeats count once
+        const int o = __builtin_amdgcn_readlane(ent, j);
+        if (j < lane && o == ent) ent = -1;
+      }
       total = len > 0 ? a.S * tpp : 0;
       return;
     }
@@ -339,15 +345,15 @@ struct KeySet {
     if (len == 0) total = 0;
   }
 
-  __device__ __forceinline__ Tile tile(const DecodeArgs& a, int64_t b, int32_t t) const {
-    if (list) {
-      const int e = t / tpp;
-      const int32_t p = list[e];
-      if (p < 0) return Tile{0, 0};
-      for (int i = 0; i < e; ++i)
-        if (list[i] == p) return Tile{0, 0};
+  // Tile t of the lane; every lane of the wave calls it.
+  __device__ __forceinline__ Tile tile(const DecodeArgs& a, int64_t b, int32_t t, bool in) const {
+    if (listed) {
+      const int e = in ? t / tpp : 0;
+      const int32_t p = __shfl(ent, e, 64);
+      if (!in || p < 0) return Tile{0, 0};
       return make_tile(a, b, (int64_t)p * a.page + (t - e * tpp) * 16, 0, len);
     }
+    if (!in) return Tile{0, 0};
     if (t < ntg) return make_tile(a, b, (int64_t)t * 16, 0, ng);
     return make_tile(a, b, wbase + (int64_t)(t - ntg) * 16, ws, len);
   }
@@ -430,7 +436,7 @@ __global__ __launch_bounds__(64 * kDecWaves, (kDecOcc<T, DP>)) void decode_kerne
   const int h0 = hk * a.G + 16 * gt;
 
   KeySet ks;
-  ks.init(a, b, hk);
+  ks.init(a, b, hk, lane);
   const int steps = (ks.total + 1) >> 1;
   const int per = (steps + a.nsplit - 1) / a.nsplit;
   const int s0 = sp * per;
@@ -554,7 +560,7 @@ __global__ __launch_bounds__(64 * kDecWaves, (kDecOcc<T, DP>)) void decode_kerne
   auto tiles = [&](int it) {
     const int step = s0 + w + kDecWaves * (it + (lane >> 1));
     const int t = 2 * step + (lane & 1);
-    td = step < s1 && t < ks.total ? ks.tile(a, b, t) : Tile{0, 0};
+    td = ks.tile(a, b, t, step < s1 && t < ks.total);
   };
   auto pick = [&](int i) {
     return Tile{__builtin_amdgcn_readlane(td.tok, i), __builtin_amdgcn_readlane(td.rng, i)};
