@@ -268,20 +268,28 @@ int ma_paged_select(const ma_paged_desc* d, const void* query, const float* key_
   (void)hipGetLastError();
   hipStream_t st = static_cast<hipStream_t>(stream);
   const size_t shm = (size_t)std::max<int64_t>(a.width, 1) * sizeof(uint64_t);
-  const dim3 grid((unsigned)(d->batch * a.Hkv)), block(kSelThreads);
-#define MA_SELECT(T)                                                                                              \
-  do {                                                                                                            \
-    if (shm > 48 * 1024 &&                                                                                        \
-        ma_host::reserve_lds(reinterpret_cast<const void*>(&page_select_kernel<T>), 16384 * sizeof(uint64_t), st)) \
-      return 1;                                                                                                   \
-    ma_host::launch(true, page_select_kernel<T>, grid, block, (uint32_t)shm, st, a);                              \
+  const dim3 grid((unsigned)(d->batch * a.Hkv));
+#define MA_SELECT(T, THREADS)                                                                                        \
+  do {                                                                                                               \
+    if (shm > 48 * 1024 && ma_host::reserve_lds(reinterpret_cast<const void*>(&page_select_kernel<T, THREADS>),      \
+                                                16384 * sizeof(uint64_t), st))                                       \
+      return 1;                                                                                                      \
+    ma_host::launch(true, page_select_kernel<T, THREADS>, grid, dim3(THREADS), (uint32_t)shm, st, a);                \
+  } while (0)
+#define MA_SELECT_W(T)             \
+  do {                             \
+    if (d->table_width > kSelWide) \
+      MA_SELECT(T, 1024);          \
+    else                           \
+      MA_SELECT(T, 512);           \
   } while (0)
   if (d->dtype == MA_ATTN_F32)
-    MA_SELECT(float);
+    MA_SELECT_W(float);
   else if (d->dtype == MA_ATTN_BF16)
-    MA_SELECT(__bf16);
+    MA_SELECT_W(__bf16);
   else
-    MA_SELECT(_Float16);
+    MA_SELECT_W(_Float16);
+#undef MA_SELECT_W
 #undef MA_SELECT
   return launched(who);
 }

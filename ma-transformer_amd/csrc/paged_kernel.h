@@ -298,11 +298,11 @@ __device__ __forceinline__ Tile make_tile(const DecodeArgs& a, int64_t b, int64_
                                           int64_t seg_hi) {
   Tile t{0, 0};
   if (seg_hi <= base || seg_lo >= base + 16) return t;
-  const int64_t l = base / a.page;
-  if (l >= a.width) return t;
+  const uint32_t l = (uint32_t)base / (uint32_t)a.page;  // base < seg_hi <= width * page < 2^31
+  if (l >= (uint32_t)a.width) return t;
   const int32_t ph = a.table[b * a.width + l];
   if (ph < 0 || ph >= a.num_pages) return t;
-  t.tok = ph * a.page + (int32_t)(base - l * a.page);
+  t.tok = ph * a.page + (int32_t)((uint32_t)base - l * (uint32_t)a.page);
   const int lo = seg_lo > base ? (int)(seg_lo - base) : 0;
   const int hi = seg_hi < base + 16 ? (int)(seg_hi - base) : 16;
   t.rng = lo | hi << 8;
@@ -694,9 +694,13 @@ __global__ __launch_bounds__(kJoinThreads) void decode_join_kernel(DecodeArgs a)
 // ---------------------------------------------------------------- page selection
 //
 // One workgroup per (stream, key/value head): eight lanes a page, the scores'
-// ordered 64-bit keys in LDS, then the num_selected largest by radix selection
-// (top_select.h).  Latency: 6 MB of page sums (32 streams of 256 pages, 4 heads)
-// would take 1.3 us, the kernel 11, most of it the selection's passes over LDS.
+// ordered 64-bit keys in LDS, then the num_selected largest (top_select.h): up to
+// 256 pages one wave with the keys in registers (against the radix passes of the
+// whole workgroup, pages scored alike: 9.9 and 11.0 us at 256 pages, 19.1 and
+// 15.8 at 512), else those passes.  Latency: 6 MB of page sums (32 streams of 256 pages, 4
+// heads of 64) would take 1.3 us, the kernel takes 6.9, and 38 for 4096 pages
+// (134 MB, 3.6 TB/s).  Four pages a lane load at once without a branch, which took
+// 11.0 to 6.9 us and 114 to 52 against a page at a time.
 
 struct SelectArgs {
   const void* q;
@@ -708,21 +712,38 @@ struct SelectArgs {
   int32_t width, page, H, Hkv, G, D, S, first, local;
 };
 
-constexpr int kSelThreads = 512;
+// Threads of a workgroup, by the table's width in pages (32 streams, 4 heads of
+// 64, full tables): 512 against 1024 threads take 6.9 and 7.6 us at 256 pages,
+// 9.8 and 10.4 at 512, 17.6 and 15.2 at 1024, 52 and 38 at 4096.
+constexpr int kSelWide = 512;  // pages
 
-template <typename T>
-__global__ __launch_bounds__(kSelThreads) void page_select_kernel(SelectArgs a) {
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void page_select_kernel(SelectArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   uint64_t* keys = reinterpret_cast<uint64_t*>(lds);
   __shared__ double s_q[128];
-  __shared__ ma_top::Scratch<kSelThreads> sc;
+  __shared__ ma_top::Scratch<THREADS> sc;
   const int tid = threadIdx.x;
   const int hk = blockIdx.x % (uint32_t)a.Hkv;
   const int64_t b = blockIdx.x / (uint32_t)a.Hkv;
   int64_t len = a.lengths[b];
   const int64_t cap = (int64_t)a.width * a.page;
   len = len < 0 ? 0 : (len > cap ? cap : len);
-  const int n = (int)((len + a.page - 1) / a.page);
+  const int n = (int)(((uint32_t)len + (uint32_t)a.page - 1) / (uint32_t)a.page);  // len <= cap < 2^31
+  // the page slots of a group's pages load before the queries' sum, and a
+  // group's sums before the products of the first
+  constexpr int kRows = THREADS / 8, kGroup = 4;
+  const int e = tid & 7, row = tid >> 3;
+  int32_t ph[kGroup];
+  auto slots = [&](int p0) {
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g) {
+      const int p = p0 + g * kRows + row;
+      ph[g] = p < n ? a.table[b * a.width + p] : -1;
+      if (ph[g] >= a.num_pages) ph[g] = -1;
+    }
+  };
+  slots(0);
   if (tid < a.D) {
     const T* qp = static_cast<const T*>(a.q) + (b * a.H + (int64_t)hk * a.G) * a.D + tid;
     double s = 0.0;
@@ -730,30 +751,55 @@ __global__ __launch_bounds__(kSelThreads) void page_select_kernel(SelectArgs a) 
     s_q[tid] = s;
   }
   __syncthreads();
-  const int e = tid & 7;
-  const int n8 = (n + kSelThreads / 8 - 1) / (kSelThreads / 8) * (kSelThreads / 8);
   const double ps = (double)a.page;
-  for (int p = tid >> 3; p < n8; p += kSelThreads / 8) {
-    int32_t ph = p < n ? a.table[b * a.width + p] : -1;
-    if (ph >= a.num_pages) ph = -1;
-    double s = 0.0;
-    if (ph >= 0) {
-      const float* x = a.sums + ((int64_t)ph * a.Hkv + hk) * a.D;
-      for (int d = 4 * e; d < a.D; d += 32) {
-        const float4 v = *reinterpret_cast<const float4*>(x + d);
-        s += (double)v.x / ps * s_q[d];
-        s += (double)v.y / ps * s_q[d + 1];
-        s += (double)v.z / ps * s_q[d + 2];
-        s += (double)v.w / ps * s_q[d + 3];
+  const bool pow2 = (a.page & (a.page - 1)) == 0;  // the product with 1 / page is the quotient
+  const double inv = 1.0 / ps;
+  const int dims = a.num_pages > 0 ? a.D : 0;
+  for (int p0 = 0; p0 < n; p0 += kGroup * kRows) {
+    if (p0) slots(p0);
+    double s[kGroup] = {};
+    for (int d = 4 * e; d < dims; d += 32) {
+      float4 v[kGroup];
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) {
+        const int64_t at = ph[g] < 0 ? 0 : ph[g];  // page 0's sums in place of none, unused
+        v[g] = *reinterpret_cast<const float4*>(a.sums + (at * a.Hkv + hk) * a.D + d);
+      }
+      const double q0 = s_q[d], q1 = s_q[d + 1], q2 = s_q[d + 2], q3 = s_q[d + 3];
+      if (pow2) {
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+          s[g] += (double)v[g].x * inv * q0;
+          s[g] += (double)v[g].y * inv * q1;
+          s[g] += (double)v[g].z * inv * q2;
+          s[g] += (double)v[g].w * inv * q3;
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+          s[g] += (double)v[g].x / ps * q0;
+          s[g] += (double)v[g].y / ps * q1;
+          s[g] += (double)v[g].z / ps * q2;
+          s[g] += (double)v[g].w / ps * q3;
+        }
       }
     }
 #pragma unroll
-    for (int k = 1; k < 8; k <<= 1) s += __shfl_xor(s, k, 64);
-    if (e == 0 && p < n)
-      keys[p] = ph < 0 ? 0 : (p < a.first || p >= n - a.local ? ~0ull : ma_top::ordered(s));
+    for (int g = 0; g < kGroup; ++g) {
+#pragma unroll
+      for (int k = 1; k < 8; k <<= 1) s[g] += __shfl_xor(s[g], k, 64);
+      const int p = p0 + g * kRows + row;
+      if (e == 0 && p < n)
+        keys[p] = ph[g] < 0 ? 0 : (p < a.first || p >= n - a.local ? ~0ull : ma_top::ordered(s[g]));
+    }
   }
   __syncthreads();
-  ma_top::list_top<kSelThreads>(keys, n, a.S, a.out + (b * a.Hkv + hk) * (int64_t)a.S, sc);
+  int32_t* out = a.out + (b * a.Hkv + hk) * (int64_t)a.S;
+  if (n <= 256) {
+    if (tid < 64) ma_top::wave_top<4>(keys, n, a.S, out);
+  } else {
+    ma_top::list_top<THREADS>(keys, n, a.S, out, sc);
+  }
 }
 
 }  // namespace ma_paged

@@ -23,6 +23,54 @@ struct Scratch {
   uint32_t wave[2][THREADS / 64];
 };
 
+// keys [n], n <= 64 R, in LDS; out [S].  Bisection from the top bit, by one wave
+// with the keys in registers: a bit stays in the threshold where S keys reach
+// it, and the search ends when exactly S do.  Equal keys go to the lowest
+// indices.  Every lane of the wave calls it.
+template <int R>
+__device__ void wave_top(const uint64_t* keys, int n, int S, int32_t* out) {
+  const int lane = threadIdx.x & 63;
+  uint64_t k[R];
+  int reach = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    k[r] = 64 * r + lane < n ? keys[64 * r + lane] : 0;
+    reach += __popcll(__ballot(k[r] != 0));
+  }
+  uint64_t least = 1;  // `reach` keys are no smaller
+  if (reach > S) {
+    least = 0;
+    for (int bit = 63; bit >= 0 && reach != S; --bit) {
+      const uint64_t t = least | 1ull << bit;
+      int c = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) c += __popcll(__ballot(k[r] >= t));
+      if (c >= S) {
+        least = t;
+        reach = c;
+      }
+    }
+  }
+  // ascending output; of the keys at the threshold the first ones
+  int above = 0;
+  if (reach > S) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) above += __popcll(__ballot(k[r] > least));
+  }
+  int ties = reach > S ? S - above : S, put = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint64_t below = (1ull << lane) - 1;
+    const uint64_t e = __ballot(k[r] == least);
+    const bool take = k[r] > least || (k[r] == least && (int)__popcll(e & below) < ties);
+    ties -= (int)__popcll(e);
+    const uint64_t b = __ballot(take);
+    if (take) out[put + __popcll(b & below)] = 64 * r + lane;
+    put += __popcll(b);
+  }
+  if (put + lane < S) out[put + lane] = -1;
+}
+
 // keys [n] in LDS; out [S].  Radix selection from the top byte: each pass
 // counts the keys that share the prefix found so far by their next byte, and
 // ends early when a bucket's end falls on S.  Equal keys go to the lowest

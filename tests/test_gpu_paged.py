@@ -467,6 +467,31 @@ def test_select_ties_and_bad_values(pa):
     assert pa.paged_select(q, cache, table, i32(*lens), 3).tolist() == [[[0, 1, 599]]]
 
 
+@pytest.mark.parametrize("width,length", [
+    (1, 1), (40, 40), (64, 64), (65, 65), (200, 200), (256, 256), (257, 257), (512, 512), (513, 513), (513, 256),
+    (513, 100), (1100, 1025), (4100, 4099),
+])
+@pytest.mark.parametrize("page", [16, 48])
+def test_select_widths(pa, page, width, length):
+    """Tables around the sizes where the kernel changes its selection and its
+    workgroup, with runs of ties, NaN, infinities and pages of the table missing;
+    pages of 48 tokens, whose quotients round."""
+    Hkv, D, n = 2, 24, (length - 1) * page + 5
+    g = torch.Generator().manual_seed(width + length + page)
+    sums = torch.randint(-3, 4, (width, Hkv, D), generator=g).float()
+    sums[torch.randint(0, width, (max(1, width // 9),), generator=g), 0, 3] = math.nan
+    sums[torch.randint(0, width, (max(1, width // 9),), generator=g), 1, 5] = -math.inf
+    table = torch.randperm(width, generator=g).to(torch.int32).view(1, width)
+    table[0, ::7] = -1
+    q = torch.zeros(1, 4, D)
+    q[0, :, 3], q[0, 2, 5], q[0, 1, 4] = 1.0, 2.0, -0.5
+    key = torch.zeros(width, page, Hkv, D, device=DEV)
+    cache = pa.PagedCache.from_tensors(key, key, sums.to(DEV))
+    for S in (1, 2, 7, 63, 64):
+        got = pa.paged_select(q.to(DEV), cache, table.to(DEV), i32(n), S)
+        assert torch.equal(got.cpu(), select64(q, sums, table, [n], page, S, 0, 1)), S
+
+
 # ---------------------------------------------------------------- together
 
 def plain_step(q, ks, vs, sel, page):
