@@ -56,8 +56,8 @@ int launched(const char* who) {
 
 // Workgroups a decode call splits its token range over: from 2048 keys on, as
 // many as fill the card (1024, four a CU).  A split costs the second launch:
-// 1024 listed keys of 32 x 4 heads take 12.4 us unsplit, 11.4 + 4.0 in two
-// parts; 65536 keys of 8 heads 24-26 us in 64 to 256 parts.  Units = (stream, kv
+// 1024 listed keys of 32 x 4 heads take 11.7 us unsplit (12.4 when two parts
+// were measured at 11.4 + 4.0); 65536 keys of 8 heads 24-26 us in 64 to 256 parts.  Units = (stream, kv
 // head, 16 query heads).
 int64_t decode_splits(const ma_paged_desc* d) {
   const int64_t G = d->num_heads / d->num_kv_heads;
