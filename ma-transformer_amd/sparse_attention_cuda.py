@@ -119,7 +119,11 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _desc_of(B, N, H, D, dtype, pattern, kw, backward=False):
-    key = (B, N, H, D, dtype, pattern, backward, tuple(sorted(kw.items())))
+    # the sizes of a set with a tile plan are in its host header, whose address
+    # (like the set's) another set may have later
+    hdr = kw.get("tile_header_ptr")
+    content = ctypes.string_at(hdr, ctypes.sizeof(_ma.TileHeader)) if hdr else b""
+    key = (B, N, H, D, dtype, pattern, backward, content, tuple(sorted(kw.items())))
     hit = _desc_cache.get(key)
     if hit is None:
         if len(_desc_cache) > 512:

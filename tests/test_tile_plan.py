@@ -131,3 +131,31 @@ def test_longformer_item_blocks():
     assert [blocks(n, 127, 0) for n in (100, 24576, 24577, 65536)] == [8, 8, 16, 16]
     assert blocks(4096, 600, 0) == 13 and blocks(65536, 600, 0) == 16
     assert blocks(4096, 5000, 5000) == blocks(65536, 5000, 5000) == 32
+
+
+def test_descriptor_cache_reads_the_header():
+    """Workspace sizes come from the tile plan's header: another set whose header,
+    plan and keys are at a freed one's addresses gets its own size."""
+    import ctypes
+
+    import ma_attn
+    import sparse_attention_cuda as ext
+    N = 513
+    i, j = np.arange(N)[:, None], np.arange(N)[None, :]
+    m = (j >= i - 40) & (j <= i + 17)
+    off = torch.from_numpy(np.concatenate([[0], np.cumsum(m.sum(1))]).astype(np.int64))
+    keys = torch.from_numpy(np.nonzero(m)[1].astype(np.int32))
+    hdr = ma_attn.TileHeader()
+    kw = dict(index_offsets_ptr=4096, index_keys_ptr=8192, num_indices=keys.numel(),
+              tile_header_ptr=ctypes.addressof(hdr), tile_plan_ptr=12288)
+    for back in (False, True):
+        bkw = dict(kw, index_t_offsets_ptr=16384, index_t_queries_ptr=20480) if back else kw
+        got = []
+        for seg in (0, 2, 0):
+            src = ma_attn.tile_header_of(off, keys, N, seg)
+            ctypes.memmove(ctypes.addressof(hdr), ctypes.addressof(src), ctypes.sizeof(hdr))
+            desc, nbytes = ext._desc_of(2, N, 2, 64, torch.bfloat16, ma_attn.INDEX_SET, bkw, backward=back)
+            size = ma_attn.backward_workspace_size if back else ma_attn.workspace_size
+            assert nbytes == size(ma_attn.make_desc(2, N, 2, 64, ma_attn.BF16, ma_attn.INDEX_SET, **bkw))
+            got.append(nbytes)
+        assert got[1] > got[0] == got[2]
